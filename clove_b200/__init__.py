@@ -12,6 +12,9 @@ def __getattr__(name):
     if name in ("KVPool", "set_decode_variant", "launch_count"):
         from . import ops
         return getattr(ops, name)
+    if name == "Fp8KVPool":
+        from . import fp8
+        return fp8.Fp8KVPool
     if name in ("CudaBackend", "PagedAttention"):
         from . import backend
         return getattr(backend, name)

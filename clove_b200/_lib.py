@@ -118,6 +118,35 @@ BLOCKS_SIGNATURES = {
 }
 
 
+class Fp8PoolInfo(C.Structure):
+    _fields_ = [("device", C.c_int), ("num_blocks", C.c_int), ("block_size", C.c_int),
+                ("num_kv_heads", C.c_int), ("head_dim", C.c_int), ("owns_memory", C.c_int),
+                ("codes", C.c_void_p), ("scales", C.c_void_p), ("mass", C.c_void_p), ("codes_bytes", C.c_size_t)]
+
+
+class Fp8Scores(C.Structure):
+    _fields_ = [("softcap", C.c_float), ("alibi_slopes", C.c_void_p), ("window", C.c_int), ("accumulate", C.c_int)]
+
+
+# include/clove_fp8.h: the 8-bit cache.
+FP8_SIGNATURES = {
+    "clove_fp8_pool_create": (_i, [_i, _i, _i, _i, _i, _i, C.POINTER(_vp)]),
+    "clove_fp8_pool_wrap": (_i, [_i, _vp, _vp, _vp, _i, _i, _i, _i, C.POINTER(_vp)]),
+    "clove_fp8_pool_destroy": (_i, [_vp]),
+    "clove_fp8_pool_info": (_i, [_vp, C.POINTER(Fp8PoolInfo)]),
+    "clove_fp8_pool_status": (_i, [_vp, _vp, _ip]),
+    "clove_fp8_append_workspace_size": (_sz, [_vp, _i]),
+    "clove_fp8_append": (_i, [_vp, _i, _vp, _vp, _vp, _i, _vp, _sz, _vp]),
+    "clove_fp8_gather": (_i, [_vp, _vp, _i, _vp, _i, _i, _vp, _vp, _vp]),
+    "clove_fp8_decode_workspace_size": (_sz, [_vp, _i, _i, _i, _i]),
+    "clove_fp8_decode": (_i, [_vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _i, _f, _i, C.POINTER(Fp8Scores), _vp, _vp,
+                              _sz, _vp]),
+    "clove_fp8_evict_workspace_size": (_sz, [_vp, _i, _i, _i]),
+    "clove_fp8_evict": (_i, [_vp, _vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _vp, _vp, _vp, _sz, _vp]),
+    "clove_fp8_copy_blocks": (_i, [_vp, _vp, _vp, _i, _vp]),
+}
+
+
 def load(path: Path | str = LIB_PATH) -> C.CDLL:
     path = Path(path)
     if not path.exists():
@@ -125,7 +154,7 @@ def load(path: Path | str = LIB_PATH) -> C.CDLL:
             f"{path} is missing: build it with `python -m clove_b200.build` "
             "(the CUDA extension is required; there is no fallback)")
     lib = C.CDLL(str(path))
-    for name, (res, args) in {**SIGNATURES, **FFI_SIGNATURES, **BLOCKS_SIGNATURES}.items():
+    for name, (res, args) in {**SIGNATURES, **FFI_SIGNATURES, **BLOCKS_SIGNATURES, **FP8_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

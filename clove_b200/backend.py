@@ -9,7 +9,8 @@ Tensors are torch CUDA tensors.  kv_cache is ONE tensor
 [2, num_blocks, block_size, num_kv_heads, head_dim] (K plane, V plane): the
 reference passes a single kv_cache and documents the per-plane layout at
 src/nn.rs:534.  q: [B, Hq*D]; k, v: [B, Hkv*D] — the new token's projections;
-context_lens: int32 [B] lengths before this token.  The call appends k, v
+context_lens: int32 [B] lengths before this token.  kv_cache may also be an
+Fp8KVPool (fp8.py): the same step over the 8-bit cache.  The call appends k, v
 through the slot mapping and attends over ctx + 1 tokens; it returns f32
 [B, Hq*D] (the reference output dtype, src/lazy.rs:5252).  context_lens is
 not modified; the caller advances it.
@@ -23,6 +24,7 @@ from collections import OrderedDict
 
 import torch
 
+from .fp8 import Fp8KVPool
 from .ops import KVPool
 
 
@@ -37,6 +39,9 @@ class CudaBackend:
 
     @classmethod
     def _pool(cls, kv_cache: torch.Tensor) -> KVPool:
+        if isinstance(kv_cache, Fp8KVPool):
+            raise TypeError("this call writes keys and values in the cache's own type: it takes a kv_cache tensor, "
+                            "not an Fp8KVPool")
         if kv_cache.dim() != 5 or kv_cache.shape[0] != 2:
             raise ValueError("kv_cache must be [2, num_blocks, block_size, num_kv_heads, head_dim]")
         key = (kv_cache.data_ptr(), tuple(kv_cache.shape), kv_cache.dtype)
@@ -51,10 +56,10 @@ class CudaBackend:
         return pool
 
     @classmethod
-    def paged_attention(cls, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor,
+    def paged_attention(cls, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor | Fp8KVPool,
                         block_tables: torch.Tensor, context_lens: torch.Tensor,
                         max_ctx: int | None = None) -> torch.Tensor:
-        pool = cls._pool(kv_cache)
+        pool = kv_cache if isinstance(kv_cache, Fp8KVPool) else cls._pool(kv_cache)
         B = context_lens.numel()
         out = pool.append_decode(q.contiguous(), k.contiguous(), v.contiguous(), block_tables, context_lens,
                                  scale=1.0 / math.sqrt(pool.head_dim), max_ctx=max_ctx)
@@ -93,7 +98,7 @@ class PagedAttention:
         self.w_o = Linear(dim, dim, device, torch.float32, g)
         self._fused: tuple[torch.Tensor, torch.Tensor] | None = None
 
-    def forward(self, x: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor,
+    def forward(self, x: torch.Tensor, kv_cache: torch.Tensor | Fp8KVPool, block_tables: torch.Tensor,
                 context_lens: torch.Tensor, max_ctx: int | None = None) -> torch.Tensor:
         q = self.w_q.forward(x)
         k = self.w_k.forward(x)

@@ -1,0 +1,244 @@
+"""Torch-facing wrapper of the 8-bit KV cache (include/clove_fp8.h): the
+counterpart of ops.KVPool whose cache holds e4m3 codes with one scale per
+(block of tokens, KV head).
+
+  codes         float8_e4m3fn [2, num_blocks, num_kv_heads, block_size, head_dim]
+  scales        float32 [2, num_blocks, num_kv_heads]; an element is code * scale
+  mass          float32 [num_blocks, num_kv_heads, block_size]: the attention
+                weight a cached token has received (optional)
+  block_tables  int32 [batch, max_blocks_per_seq]
+  context_lens  int32 [batch]
+  q, k, v       float32, bfloat16 or float16
+  out           float32 [batch, num_q_heads, head_dim]
+
+No counterpart in the reference, whose kv_cache is f32 (src/nn.rs:534).
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+import math
+
+import torch
+
+from . import _lib
+from .ops import _DTYPES, _ptr
+
+
+class Fp8KVPool:
+    """A paged 8-bit KV cache on one GPU.  `storage`, `scales` and `mass` wrap
+    the caller's tensors; what is missing is allocated (mass only with
+    track_mass).  Blocks are filled from row 0 on: a write to row 0 starts a
+    block anew, whatever an earlier sequence left in it.
+
+    Scratch comes from the caching allocator call by call, so calls on
+    different streams, and graphs captured from them, share none."""
+
+    def __init__(self, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
+                 device: int | torch.device = 0, storage: torch.Tensor | None = None,
+                 scales: torch.Tensor | None = None, mass: torch.Tensor | None = None, track_mass: bool = False):
+        self.device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        if self.device.type != "cuda":
+            raise ValueError("Fp8KVPool lives on a CUDA device")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        shapes = {"storage": ((2, num_blocks, num_kv_heads, block_size, head_dim), torch.float8_e4m3fn),
+                  "scales": ((2, num_blocks, num_kv_heads), torch.float32),
+                  "mass": ((num_blocks, num_kv_heads, block_size), torch.float32)}
+        for name, t in (("storage", storage), ("scales", scales), ("mass", mass)):
+            shape, dtype = shapes[name]
+            if t is not None and (tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous()
+                                  or t.device != self.device):
+                raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {self.device}")
+        if (storage is None) != (scales is None):
+            raise ValueError("storage and scales go together")
+        if storage is None:
+            storage = torch.zeros(shapes["storage"][0], dtype=torch.uint8, device=self.device).view(torch.float8_e4m3fn)
+            scales = torch.zeros(shapes["scales"][0], dtype=torch.float32, device=self.device)
+        if mass is None and track_mass:
+            mass = torch.zeros(shapes["mass"][0], dtype=torch.float32, device=self.device)
+        self.storage, self.scales, self.mass = storage, scales, mass
+        self.num_blocks, self.block_size = num_blocks, block_size
+        self.num_kv_heads, self.head_dim = num_kv_heads, head_dim
+        self._lib = _lib.lib()
+        h = C.c_void_p()
+        _lib.check(self._lib.clove_fp8_pool_wrap(self.device.index, _ptr(storage), _ptr(scales), _ptr(mass),
+                                                 num_blocks, block_size, num_kv_heads, head_dim, C.byref(h)))
+        self.handle = h
+
+    def close(self) -> None:
+        if getattr(self, "handle", None):
+            self._lib.clove_fp8_pool_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    # ---- checks ------------------------------------------------------------
+    @contextlib.contextmanager
+    def _on(self, stream: torch.cuda.Stream | None):
+        """The stream of a call: what the call allocates or copies belongs to
+        it, whichever device and stream are current."""
+        if stream is not None and stream.device != self.device:
+            raise ValueError(f"stream is on {stream.device}, the pool on {self.device}")
+        if stream is None and torch.cuda.current_device() == self.device.index:
+            yield torch.cuda.current_stream().cuda_stream
+            return
+        s = stream if stream is not None else torch.cuda.current_stream(self.device)
+        with torch.cuda.stream(s):
+            yield s.cuda_stream
+
+    def _rows(self, t: torch.Tensor, rows: int, heads: int, name: str, dtype: torch.dtype | None = None) -> torch.Tensor:
+        if t.device != self.device or t.dtype not in _DTYPES or (dtype is not None and t.dtype != dtype):
+            want = dtype if dtype is not None else "float32, bfloat16 or float16"
+            raise ValueError(f"{name} must be a {want} tensor on {self.device}")
+        if t.numel() != rows * heads * self.head_dim:
+            raise ValueError(f"{name} must hold {rows} x {heads} x {self.head_dim} elements, not {tuple(t.shape)}")
+        t = t.reshape(rows, heads, self.head_dim).contiguous()
+        return t if t.data_ptr() % 16 == 0 else t.clone()
+
+    def _i32(self, t: torch.Tensor, name: str, dim: int, rows: int | None = None) -> torch.Tensor:
+        if t.dtype != torch.int32 or t.device != self.device or t.dim() != dim or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dim}-D int32 tensor on {self.device}")
+        if rows is not None and t.shape[0] != rows:
+            raise ValueError(f"{name} has {t.shape[0]} rows, not {rows}")
+        return t
+
+    def _scratch(self, n: int) -> torch.Tensor | None:
+        return torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+
+    def _max_ctx(self, context_lens: torch.Tensor, max_ctx: int | None, extra: int = 0) -> int:
+        if max_ctx is None:  # forces a device sync; pass it on hot paths
+            return int(context_lens.max().item()) + extra if context_lens.numel() else 0
+        return int(max_ctx)
+
+    # ---- ops ---------------------------------------------------------------
+    def reshape_and_cache(self, k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor,
+                          stream: torch.cuda.Stream | None = None) -> None:
+        """Quantise k, v [num_tokens, num_kv_heads, head_dim] into the slots
+        slot_mapping (int32 [num_tokens]; negative: padding, skipped).  A
+        block's scale grows to cover what is written and the rows already in
+        it are rounded to it; a write to row 0 starts the block anew."""
+        with self._on(stream) as s:
+            self._i32(slot_mapping, "slot_mapping", 1)
+            n = slot_mapping.numel()
+            k = self._rows(k, n, self.num_kv_heads, "k")
+            v = self._rows(v, n, self.num_kv_heads, "v", k.dtype)
+            ws = self._scratch(self._lib.clove_fp8_append_workspace_size(self.handle, n))
+            _lib.check(self._lib.clove_fp8_append(self.handle, _DTYPES[k.dtype], _ptr(k), _ptr(v), _ptr(slot_mapping), n,
+                                                  _ptr(ws), ws.numel() if ws is not None else 0, s))
+
+    def gather_kv(self, block_tables: torch.Tensor, context_lens: torch.Tensor, max_ctx: int,
+                  stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """The cached tokens as float32 [batch, max_ctx, num_kv_heads,
+        head_dim]; rows behind a sequence's last token are zero."""
+        with self._on(stream) as s:
+            self._i32(context_lens, "context_lens", 1)
+            b = context_lens.numel()
+            self._i32(block_tables, "block_tables", 2, b)
+            shape = (b, max_ctx, self.num_kv_heads, self.head_dim)
+            ko = torch.empty(shape, dtype=torch.float32, device=self.device)
+            vo = torch.empty(shape, dtype=torch.float32, device=self.device)
+            _lib.check(self._lib.clove_fp8_gather(self.handle, _ptr(block_tables), block_tables.shape[1],
+                                                  _ptr(context_lens), b, max_ctx, _ptr(ko), _ptr(vo), s))
+            return ko, vo
+
+    def decode(self, q: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
+               scale: float | None = None, max_ctx: int | None = None, out: torch.Tensor | None = None,
+               k_new: torch.Tensor | None = None, v_new: torch.Tensor | None = None, softcap: float = 0.0,
+               alibi_slopes: torch.Tensor | None = None, window: int = 0, accumulate: bool = False,
+               stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+        """Decode over the cache; with k_new/v_new the new token is appended
+        first (context_lens are then the lengths before it, max_ctx bounds
+        those after it).  Scores, in this order: softcap * tanh(. / softcap);
+        + alibi_slopes[hq] * (t - (L - 1)) with float32 [num_q_heads] slopes;
+        only the last `window` tokens.  accumulate adds each token's weight,
+        summed over its KV head's query heads, to the pool's mass."""
+        with self._on(stream) as s:
+            self._i32(context_lens, "context_lens", 1)
+            batch = context_lens.numel()
+            self._i32(block_tables, "block_tables", 2, batch)
+            hq = q.shape[1] // self.head_dim if q.dim() == 2 else q.shape[1]
+            q = self._rows(q, batch, hq, "q")
+            append = k_new is not None
+            if append != (v_new is not None):
+                raise ValueError("k_new and v_new go together")
+            if append:
+                k_new = self._rows(k_new, batch, self.num_kv_heads, "k_new", q.dtype)
+                v_new = self._rows(v_new, batch, self.num_kv_heads, "v_new", q.dtype)
+            if alibi_slopes is not None and (alibi_slopes.shape != (hq,) or alibi_slopes.dtype != torch.float32
+                                             or alibi_slopes.device != self.device
+                                             or not alibi_slopes.is_contiguous()):
+                raise ValueError(f"alibi_slopes must be a contiguous float32 [{hq}] tensor on {self.device}")
+            if accumulate and self.mass is None:
+                raise ValueError("accumulate needs a pool with mass (track_mass=True)")
+            max_ctx = self._max_ctx(context_lens, max_ctx, int(append))
+            shape = (batch, hq, self.head_dim)
+            if out is None:
+                out = torch.empty(shape, dtype=torch.float32, device=self.device)
+            elif tuple(out.shape) != shape or out.dtype != torch.float32 or out.device != self.device \
+                    or not out.is_contiguous():
+                raise ValueError(f"out must be a contiguous float32 tensor of shape {shape} on {self.device}")
+            scores = _lib.Fp8Scores(float(softcap), _ptr(alibi_slopes), int(window), int(bool(accumulate)))
+            ws = self._scratch(self._lib.clove_fp8_decode_workspace_size(self.handle, batch, hq, max_ctx,
+                                                                         int(bool(accumulate))))
+            _lib.check(self._lib.clove_fp8_decode(
+                self.handle, _DTYPES[q.dtype], _ptr(q), _ptr(k_new), _ptr(v_new), hq, _ptr(block_tables),
+                block_tables.shape[1], _ptr(context_lens), batch,
+                1.0 / math.sqrt(self.head_dim) if scale is None else float(scale), max_ctx, C.byref(scores), _ptr(out),
+                _ptr(ws), ws.numel() if ws is not None else 0, s))
+            return out
+
+    def append_decode(self, q, k_new, v_new, block_tables, context_lens, **kw) -> torch.Tensor:
+        return self.decode(q, block_tables, context_lens, k_new=k_new, v_new=v_new, **kw)
+
+    def evict(self, block_tables: torch.Tensor, context_lens: torch.Tensor, new_tables: torch.Tensor, budget: int,
+              recent: int = 0, max_ctx: int | None = None,
+              stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Bring every sequence down to min(context_lens, budget) tokens: each
+        KV head keeps the last `recent` ones and the heaviest others (mass;
+        ties to the lower index), moved in order to the blocks new_tables,
+        which must be none of the blocks the sequences hold now.  Returns
+        (kept int32 [batch, num_kv_heads, budget], -1 behind the last,
+        new_lens int32 [batch]).  Token indices are those of the compacted
+        cache from then on (windows and distance biases count in them)."""
+        with self._on(stream) as s:
+            self._i32(context_lens, "context_lens", 1)
+            batch = context_lens.numel()
+            self._i32(block_tables, "block_tables", 2, batch)
+            self._i32(new_tables, "new_tables", 2, batch)
+            if self.mass is None:
+                raise ValueError("evict needs a pool with mass (track_mass=True)")
+            budget, recent = int(budget), int(recent)
+            if budget < 1 or not 0 <= recent <= budget:
+                raise ValueError(f"budget {budget}, recent {recent}: 0 <= recent <= budget, budget >= 1")
+            max_ctx = self._max_ctx(context_lens, max_ctx)
+            kept = torch.empty((batch, self.num_kv_heads, budget), dtype=torch.int32, device=self.device)
+            lens = torch.empty(batch, dtype=torch.int32, device=self.device)
+            ws = self._scratch(self._lib.clove_fp8_evict_workspace_size(self.handle, batch, max_ctx, budget))
+            _lib.check(self._lib.clove_fp8_evict(
+                self.handle, _ptr(block_tables), block_tables.shape[1], _ptr(context_lens), batch, max_ctx,
+                _ptr(new_tables), new_tables.shape[1], budget, recent, _ptr(kept), _ptr(lens), _ptr(ws),
+                ws.numel() if ws is not None else 0, s))
+            return kept, lens
+
+    def copy_blocks(self, src: torch.Tensor, dst: torch.Tensor, stream: torch.cuda.Stream | None = None) -> None:
+        """Copy blocks src[i] -> dst[i] (int32 device tensors): the block
+        manager's copy-on-write copies."""
+        with self._on(stream) as s:
+            self._i32(src, "src", 1)
+            self._i32(dst, "dst", 1, src.numel())
+            _lib.check(self._lib.clove_fp8_copy_blocks(self.handle, _ptr(src), _ptr(dst), src.numel(), s))
+
+    def pool_status(self, stream: torch.cuda.Stream | None = None) -> int:
+        """Check flags (FLAG_*) that the pool's calls raised since the last
+        read; synchronises the stream."""
+        flags = C.c_int(0)
+        with self._on(stream) as s:
+            rc = self._lib.clove_fp8_pool_status(self.handle, s, C.byref(flags))
+        if rc not in (_lib.OK, _lib.ERR_DEVICE_CHECK):
+            _lib.check(rc)
+        return flags.value
