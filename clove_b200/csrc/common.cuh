@@ -220,6 +220,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 __host__ __device__ constexpr int state_stride(int head_dim) { return head_dim + 4; }
 
 struct DecodeArgs {
+  // what the combine and the merge do beside the outputs (an Args type derived
+  // from this one may differ)
+  static constexpr bool kPublishFlags = true;    // the combine moves err to err_last
+  static constexpr bool kKeepsRowState = false;  // (M, 1 / L) of every output row is kept in row_state
   const void* q;             // [B, Hq, D] pool dtype
   const void* k_new;         // [B, Hkv, D] or null (no append)
   const void* v_new;

@@ -549,8 +549,8 @@ __device__ __forceinline__ bool wait_or_abort(const DecodeArgs& a, const SmemPtr
 // 16-byte loads.  A complete segment is finished here (out = sum f acc / L);
 // a split one leaves its merged state (sum f acc, M, L) in the CTA's partial
 // slot [num_ctas, 2, group, S] for the combine kernel.
-template <int D, int G, int NW>
-__device__ void merge_unit(const DecodeArgs& a, const Unit& x, const float* scratch, int lane) {
+template <int D, int G, int NW, typename Args>
+__device__ void merge_unit(const Args& a, const Unit& x, const float* scratch, int lane) {
   constexpr int S = state_stride(D);
   static_assert(G * NW <= 32, "one lane per (row, warp) state");
   const int group = a.group;
@@ -581,6 +581,10 @@ __device__ void merge_unit(const DecodeArgs& a, const Unit& x, const float* scra
     const float Lg = __shfl_sync(0xffffffffu, Lr, g * NW);
     const float Mg = __shfl_sync(0xffffffffu, M, g * NW);
     const float inv = 1.f / Lg;
+    if constexpr (Args::kKeepsRowState) {
+      if (a.row_state != nullptr && x.complete && lane == 0)
+        a.row_state[(size_t)x.b * Hq + x.h * group + g] = make_float2(Mg, inv);
+    }
     for (int d4 = lane; d4 < D / 4; d4 += 32) {
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -617,8 +621,8 @@ __device__ void merge_unit(const DecodeArgs& a, const Unit& x, const float* scra
 // scratch buffer sbuf: release the unit slot, count the warp in, and if it
 // is the last of the NW warps, merge the piece and free the buffer.  No warp
 // waits for another here.
-template <int D, int G, int NW>
-__device__ __forceinline__ void hand_off(const DecodeArgs& a, const SmemPtrs& sm, const UnitSlot& us, int sbuf,
+template <int D, int G, int NW, typename Args>
+__device__ __forceinline__ void hand_off(const Args& a, const SmemPtrs& sm, const UnitSlot& us, int sbuf,
                                          int uk, int lane) {
   __syncwarp();
   int last = 0;

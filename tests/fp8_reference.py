@@ -67,7 +67,12 @@ class RefPool:
         largest sum of magnitudes (scale * sum |q k|, plus the bias).  That is
         the weight's relative error, met once in the numerator and once in the
         denominator; exp2, the split of a weight into two halves and the
-        sums over L tokens add (L / 32 + 24) 2^-23."""
+        sums over L tokens add (L / 32 + 24) 2^-23.  A weight is held as two
+        f16 numbers in units in which the row's largest is 2^14 or more and
+        the block's scale is relative to the largest scale s_max: whatever is
+        below f16's smallest step, 2^-24, is rounded, which is at most 2^-25,
+        so a token adds at most 2^-39 s_max |code| (of the row's largest
+        weight, which is at most 1) to an output that it may be light in."""
         q = q.cpu().double()
         B, hq, D = q.shape
         H = self.codes.shape[2]
@@ -80,6 +85,7 @@ class RefPool:
             pos = torch.arange(max(0, L - window) if window else 0, L)
             k, v = (self.rows(p, tables[b].cpu(), pos) for p in range(2))
             blk = tables[b].cpu().long()[pos // self.bs]
+            s_max = self.scales[1][blk].amax(0)
             for h in range(H):
                 g0, g1 = h * (hq // H), (h + 1) * (hq // H)
                 z = scale * q[b, g0:g1] @ k[:, h].t()
@@ -93,7 +99,8 @@ class RefPool:
                 p = torch.softmax(z, 1)
                 rel = 2 * (D / 16 + 8) * 2.0 ** -23 * S + (L / 32 + 24) * 2.0 ** -23
                 out[b, g0:g1] = p @ v[:, h]
-                bound[b, g0:g1] = rel[:, None] * (p @ v[:, h].abs()) + 1e-37
+                bound[b, g0:g1] = rel[:, None] * (p @ v[:, h].abs()) + 1e-37 + \
+                    2.0 ** -39 * s_max[h] * self.codes[1][blk, h, pos % self.bs].abs().sum(0)
                 if accumulate:
                     self.mass[blk, h, pos % self.bs] += p.sum(0)
                     self.mass_bound[blk, h, pos % self.bs] += (rel[:, None] * p).sum(0) + 2.0 ** -23 * p.sum(0)
