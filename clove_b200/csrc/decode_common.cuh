@@ -166,7 +166,9 @@ __device__ __forceinline__ SmemPtrs smem_ptrs(unsigned char* base, const SmemPla
 }
 
 // Barrier initialisation (thread 0), then a CTA barrier.  ncw_all: consumer
-// warps in the CTA (each arrives on uempty once per unit).
+// warps in the CTA (each arrives on uempty once per unit).  SCR0, SCR1: the
+// arrivals that complete a phase of scr_empty[0] and [1].
+template <int SCR0 = 1, int SCR1 = 1>
 __device__ __forceinline__ void init_barriers(const SmemPtrs& p, int nstage, int ncw_all) {
   if (threadIdx.x == 0) {
     for (int s = 0; s < nstage; ++s) {
@@ -177,8 +179,8 @@ __device__ __forceinline__ void init_barriers(const SmemPtrs& p, int nstage, int
       mbar_init(&p.ufull[k], 1);
       mbar_init(&p.uempty[k], ncw_all);
     }
-    mbar_init(&p.scr_empty[0], 1);
-    mbar_init(&p.scr_empty[1], 1);
+    mbar_init(&p.scr_empty[0], SCR0);
+    mbar_init(&p.scr_empty[1], SCR1);
     p.misc[0] = 0;
     p.arrive[0] = 0;
     p.arrive[1] = 0;
@@ -549,8 +551,8 @@ __device__ __forceinline__ bool wait_or_abort(const DecodeArgs& a, const SmemPtr
 // 16-byte loads.  A complete segment is finished here (out = sum f acc / L);
 // a split one leaves its merged state (sum f acc, M, L) in the CTA's partial
 // slot [num_ctas, 2, group, S] for the combine kernel.
-template <int D, int G, int NW, typename Args>
-__device__ void merge_unit(const Args& a, const Unit& x, const float* scratch, int lane) {
+template <int D, int G, int NW>
+__device__ void merge_unit(const DecodeArgs& a, const Unit& x, const float* scratch, int lane) {
   constexpr int S = state_stride(D);
   static_assert(G * NW <= 32, "one lane per (row, warp) state");
   const int group = a.group;
@@ -581,10 +583,6 @@ __device__ void merge_unit(const Args& a, const Unit& x, const float* scratch, i
     const float Lg = __shfl_sync(0xffffffffu, Lr, g * NW);
     const float Mg = __shfl_sync(0xffffffffu, M, g * NW);
     const float inv = 1.f / Lg;
-    if constexpr (Args::kKeepsRowState) {
-      if (a.row_state != nullptr && x.complete && lane == 0)
-        a.row_state[(size_t)x.b * Hq + x.h * group + g] = make_float2(Mg, inv);
-    }
     for (int d4 = lane; d4 < D / 4; d4 += 32) {
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -621,8 +619,8 @@ __device__ void merge_unit(const Args& a, const Unit& x, const float* scratch, i
 // scratch buffer sbuf: release the unit slot, count the warp in, and if it
 // is the last of the NW warps, merge the piece and free the buffer.  No warp
 // waits for another here.
-template <int D, int G, int NW, typename Args>
-__device__ __forceinline__ void hand_off(const Args& a, const SmemPtrs& sm, const UnitSlot& us, int sbuf,
+template <int D, int G, int NW>
+__device__ __forceinline__ void hand_off(const DecodeArgs& a, const SmemPtrs& sm, const UnitSlot& us, int sbuf,
                                          int uk, int lane) {
   __syncwarp();
   int last = 0;

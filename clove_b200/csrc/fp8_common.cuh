@@ -21,7 +21,7 @@ struct clove_fp8_pool {
   size_t plane_bytes;    // bytes of one plane of codes
   int32_t* flags;        // device word: check flags of all calls
   int num_sms;
-  CUtensorMap tm_k, tm_v;  // the planes as the decode's copies see them
+  CUtensorMap map;  // the codes as the decode's copies see them
 };
 
 namespace clove {
@@ -131,7 +131,7 @@ int launch_fp8_gather(const clove_fp8_pool& pool, const int32_t* block_tables, i
                       const int32_t* context_lens, int batch, int max_ctx, float* k_out, float* v_out,
                       cudaStream_t stream);
 int launch_fp8_copy(const clove_fp8_pool& pool, const int32_t* src, const int32_t* dst, int n, cudaStream_t stream);
-int fp8_encode_maps(clove_fp8_pool& pool);
+int fp8_encode_map(clove_fp8_pool& pool);
 size_t fp8_decode_workspace(const clove_fp8_pool& pool, int batch, int num_q_heads, int max_ctx, int accumulate);
 int launch_fp8_decode(const clove_fp8_pool& pool, const Fp8DecodeCall& call, cudaStream_t stream);
 size_t fp8_evict_workspace(const clove_fp8_pool& pool, int batch, int max_ctx, int budget);

@@ -3,29 +3,34 @@
 // The work partition, the pipeline (one producer warp, a ring of stages in
 // shared memory, consumer warps that own whole stages), the merge and the
 // combine are those of the other decodes (decode_common.cuh, combine.cuh).
-// The unit of the partition is a slice of up to 32 tokens of one (block, KV
-// head) tile: kSlice = min(block_size, 32), so a block of 256 tokens is eight
-// slices with one scale.
+// The unit of the partition is a slice of one (block, KV head) tile: the tile,
+// or the part of it that fills a stage (16 KB of K and V: 64 tokens at head_dim
+// 128), so a block of 256 such tokens is four slices with one scale.
 //
 // Mathematics.  HBM bounds this kernel, so the arithmetic is held to what
 // float32 would give instead of spending the slack elsewhere:
 //   - an e4m3 code is exact in f16, so K and V enter the tensor cores exactly,
 //     and their block scales are applied to scores and weights in f32;
-//   - a query element is the sum of two halves (f16 queries and, but for
-//     elements 2^-31 below the row's largest, bf16 queries are one half), a
-//     weight the sum of two halves.  The m16n8k16 MMA has 16 rows and a KV
-//     head at most 8 queries: the high halves are rows 0..7, the low halves
+//   - scores are computed transposed, K (16 tokens) times Q^T (8 queries): the
+//     m16n8k16 MMA has no row to spare.  A 16-bit query is one half once its
+//     row is scaled to the top of the f16 range (bf16 elements 2^-31 below the
+//     row's largest lose bits), an f32 query the sum of two halves and so two
+//     MMAs;
+//   - a weight is the sum of two halves.  In P.V the queries are the MMA's
+//     rows, at most 8 of 16: the high halves are rows 0..7, the low halves
 //     rows 8..15 of the same instruction, and the two results meet in one
-//     thread's registers;
+//     thread's registers.  An 8x8 transpose of f16 pairs (movmatrix) turns the
+//     score fragment into that operand;
 //   - weights are 2^(z - m + 14): the f16 range below the largest weight is 14
 //     binades longer than with 2^(z - m), so a weight is off by at most 2^-39
 //     of the row's largest however many light tokens there are;
 //   - the scales of V differ from block to block: a warp keeps the largest
 //     power of two seen, `vref`, in its accumulators' unit (as it keeps the
 //     running maximum m), and multiplies weights by v_scale / vref <= 2;
-//   - the value sum of 32 tokens starts from zero in the tensor cores and is
-//     added to f32 registers, so the chain of truncated tensor-core additions
-//     is two long, not as long as the sequence.
+//   - the value sum of a pass (64 tokens; 32 for head_dim 256) starts from zero
+//     in the tensor cores and is added to f32 registers, so the chain of
+//     truncated tensor-core additions is four long, not as long as the
+//     sequence.
 //
 // Shared memory.  A tile is contiguous in HBM; it is copied as rows of 128
 // bytes (64 for head_dim 64) with the hardware swizzle: the 16-byte chunk at
@@ -35,12 +40,14 @@
 #include <algorithm>
 #include <cstdlib>
 #include <mutex>
+#include <type_traits>
 #include <unordered_map>
 
 #include "combine.cuh"
 #include "common.cuh"
 #include "decode_common.cuh"
 #include "fp8_common.cuh"
+#include "mma_common.cuh"
 
 namespace clove {
 
@@ -54,38 +61,28 @@ struct Fp8Args : DecodeArgs {
   float* z;            // [batch, Hq, z_stride]: scores in the log2 domain (accumulate only, else null)
   long long z_stride;
   int real_block;      // tokens per cache block; DecodeArgs::block_size is the slice
-  int sub_shift;       // log2(real_block / slice)
+  int slice_shift;     // log2 of the slice
+  int real_shift;      // log2 of real_block
   int window;
   int append_here;     // 1: the producers append the new tokens (see fp8_append_kernel)
   int direct;          // 1: CTA c takes segment c whole, nothing is split
   float scale, softcap;
 };
 
-constexpr int kSlice = 32;
-constexpr int kMaxSb = 16;  // slices per stage: 128 tokens of 8 (head_dim 64)
+constexpr int kSclRing = 128;  // slices whose scales the ring holds (see fp8_produce)
 
 // Stage tokens: 16 KB of K and V.
-template <int D>
-constexpr int stage_tokens() {
-  return D == 64 ? 128 : D == 128 ? 64 : 32;
-}
-
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
-                                            uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
-      " [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar)), "l"(policy)
-      : "memory");
-}
+constexpr int stage_tokens(int head_dim) { return 8192 / head_dim; }
 
 // First slice of sequence b that the call reads.
 __device__ __forceinline__ int first_slice(const Fp8Args& a, int L) {
-  return a.window > 0 ? max(0, L - a.window) / a.block_size : 0;
+  return a.window > 0 ? max(0, L - a.window) >> a.slice_shift : 0;
 }
 __device__ __forceinline__ int num_slices(const Fp8Args& a, int L) {
-  return (L + a.block_size - 1) / a.block_size - first_slice(a, L);
+  return ((L + a.block_size - 1) >> a.slice_shift) - first_slice(a, L);
 }
+
+__device__ __noinline__ unsigned long long udiv64(unsigned long long a, unsigned b) { return a / b; }
 
 // partition_prologue (decode_common.cuh) for segments that start at a window.
 template <int D>
@@ -132,15 +129,18 @@ __device__ void fp8_prologue(const Fp8Args& a, WalkStart* out) {
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   if (lane == 0 && mine) atomicAdd(reinterpret_cast<unsigned long long*>(&s_sum), (unsigned long long)mine);
   __syncthreads();
-  const long long W = s_sum * H, P = a.num_ctas;
-  const long long lo = range_begin(blockIdx.x, W, P), hi = range_begin(blockIdx.x + 1, W, P);
+  // floor(c W / P) = c (W / P) + floor(c (W mod P) / P), the last in 32 bits
+  const unsigned long long W = (unsigned long long)s_sum * H, quot = udiv64(W, a.num_ctas);
+  const unsigned rest = (unsigned)(W - quot * a.num_ctas), c = blockIdx.x;
+  const long long lo = (long long)(c * quot + c * rest / a.num_ctas);
+  const long long hi = (long long)((c + 1) * quot + (c + 1) * rest / a.num_ctas);
   if (tid == 0) {
     out->lo = lo;
     out->hi = hi;
     out->b = -1;
     out->h = 0;
     out->off = 0;
-    if (blockIdx.x == 0) *a.total = W;
+    if (blockIdx.x == 0) *a.total = (long long)W;
   }
   if (lo < hi) {
     long long carry = 0;
@@ -152,10 +152,10 @@ __device__ void fp8_prologue(const Fp8Args& a, WalkStart* out) {
       const int excl = block_excl_scan(len, warp_tot, &tot);
       const long long s0 = (carry + excl) * H;
       if (len > 0 && s0 <= lo && lo < s0 + (long long)len * H) {
-        const long long r = lo - s0;
+        const unsigned long long r = lo - s0, hh = udiv64(r, len);
         out->b = b;
-        out->h = (int)(r / len);
-        out->off = (int)(r - (r / len) * len);
+        out->h = (int)hh;
+        out->off = (int)(r - hh * len);
         s_found = 1;
       }
       carry += tot;
@@ -173,57 +173,77 @@ __device__ void fp8_prologue(const Fp8Args& a, WalkStart* out) {
   }
 }
 
-// The new token of head h: settles the block's scale with the row, rounds the
-// rows already there if it grew, writes the row.  One warp, D / 8 lanes hold
-// the row; nobody else reads or writes this tile before the copies that the
-// caller issues next.
+// The new token of one (sequence, KV head), held by a warp: lanes 0..15 have
+// its K row, lanes 16..31 its V row, D / 16 elements each.
+template <int D>
+struct NewRow {
+  int phys;   // its block, -1: none
+  float old;  // the plane's scale before it, after fp8_store_new the scale now
+  float v[D / 16];
+};
+
 template <typename T, int D>
-__device__ void fp8_append_row(const Fp8Args& a, int b, int h, int L, int lane) {
-  const int bs = a.real_block, H = a.num_kv_heads, pos = L - 1, off = pos & (bs - 1);
-  const int phys = __ldg(a.block_tables + (size_t)b * a.bt_stride + pos / bs);
+__device__ __forceinline__ void fp8_load_new(const Fp8Args& a, int b, int h, int L, int phys, int lane, NewRow<D>& n) {
+  const int off = (L - 1) & (a.real_block - 1), H = a.num_kv_heads, p = lane >> 4;
+  n.phys = phys;
   if (phys < 0 || phys >= a.num_blocks) {
     if (lane == 0) atomicOr(a.err, CLOVE_FLAG_BLOCK_OOB);
+    n.phys = -1;
     return;
   }
-  const size_t tile = (size_t)phys * H + h, src = ((size_t)b * H + h) * D + lane * 8;
-  float v[2][8] = {};
-  float old[2];
-  if (lane < D / 8) {
-    load_vec_f32<T, 8>(static_cast<const T*>(a.k_new) + src, v[0]);
-    load_vec_f32<T, 8>(static_cast<const T*>(a.v_new) + src, v[1]);
+  n.old = off == 0 ? 0.f : __ldcg(a.scales + ((size_t)p * a.num_blocks + phys) * H + h);
+  const T* src = static_cast<const T*>(p ? a.v_new : a.k_new) + ((size_t)b * H + h) * D + (lane & 15) * (D / 16);
+#pragma unroll
+  for (int i = 0; i < D / 16; i += 4) load_vec_f32<T, 4>(src + i, reinterpret_cast<float(&)[4]>(n.v[i]));
+}
+
+// 1 / s: exact for the powers of two that scales are.
+__device__ __forceinline__ float fp8_inverse(float s) { return __frcp_rn(s); }
+
+// Rounds a tile's codes, but for row `but`, to a scale 1 / ratio times as
+// large.  Sixteen lanes; out of line, for it is rare.
+__device__ __noinline__ void fp8_rescale_tile(unsigned char* rows, int chunks, int chunks_per_row, int but, float ratio,
+                                              int lane) {
+  uint4* w = reinterpret_cast<uint4*>(rows);
+#pragma unroll 1
+  for (int i = lane; i < chunks; i += 16) {
+    if (i / chunks_per_row == but) continue;
+    const uint4 c = __ldcg(w + i);
+    const uint2 lo = fp8_rescale8(make_uint2(c.x, c.y), ratio), hi = fp8_rescale8(make_uint2(c.z, c.w), ratio);
+    w[i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
   }
+}
+
+// Settles the block's scale with the row, rounds the rows already there if it
+// grew, writes the row.  Nobody else reads or writes this tile before the
+// copies that the caller issues next.  The new scales come back in n.old.
+template <int D>
+__device__ __forceinline__ void fp8_store_new(const Fp8Args& a, int h, int L, int lane, NewRow<D>& n) {
+  if (n.phys < 0) return;
+  const int bs = a.real_block, H = a.num_kv_heads, off = (L - 1) & (bs - 1), p = lane >> 4;
+  const size_t tile = (size_t)n.phys * H + h;
+  float amax = 0.f;
 #pragma unroll
-  for (int p = 0; p < 2; ++p) old[p] = off == 0 ? 0.f : __ldcg(a.scales + (size_t)p * a.num_blocks * H + tile);
+  for (int i = 0; i < D / 16; ++i) amax = fmaxf(amax, finite_abs(n.v[i]));
 #pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    float amax = 0.f;
+  for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  const float s = fmaxf(n.old, fp8_scale_for(amax)), inv = fp8_inverse(s);
+  unsigned char* rows = static_cast<unsigned char*>(p ? a.v_cache : a.k_cache) + tile * bs * D;
+  if (n.old > 0.f && s > n.old)  // the row itself is written below
+    fp8_rescale_tile(rows, bs * (D / 16), D / 16, off, n.old / s, lane & 15);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(rows + (size_t)off * D + (lane & 15) * (D / 16));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, finite_abs(v[p][i]));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const float s = fmaxf(old[p], fp8_scale_for(amax)), inv = 1.f / s;
-    unsigned char* rows = static_cast<unsigned char*>(p ? a.v_cache : a.k_cache) + tile * bs * D;
-    if (old[p] > 0.f && s > old[p]) {
-      const float ratio = old[p] / s;
-      uint4* w = reinterpret_cast<uint4*>(rows);
-#pragma unroll 4
-      for (int i = lane; i < bs * (D / 16); i += 32) {
-        if (i / (D / 16) == off) continue;  // written below
-        const uint4 c = __ldcg(w + i);
-        const uint2 lo = fp8_rescale8(make_uint2(c.x, c.y), ratio), hi = fp8_rescale8(make_uint2(c.z, c.w), ratio);
-        w[i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-      }
-    }
-    if (lane < D / 8) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[p][i] *= inv;
-      *reinterpret_cast<uint2*>(rows + (size_t)off * D + lane * 8) = fp8_pack8(v[p]);
-    }
-    if (lane == 0) a.scales[(size_t)p * a.num_blocks * H + tile] = s;
-  }
+  for (int i = 0; i < D / 16; i += 4)
+    dst[i / 4] = fp8_pack2(n.v[i] * inv, n.v[i + 1] * inv) | fp8_pack2(n.v[i + 2] * inv, n.v[i + 3] * inv) << 16;
+  if ((lane & 15) == 0) a.scales[(size_t)p * a.num_blocks * H + tile] = s;
+  n.old = s;
   if (lane == 0 && a.mass != nullptr && a.z == nullptr) a.mass[tile * bs + off] = 0.f;
   fence_proxy_async_global();
   __syncwarp();
+}
+
+__device__ __forceinline__ int new_entry(const Fp8Args& a, int b, int L) {
+  return __ldg(a.block_tables + (size_t)b * a.bt_stride + ((L - 1) >> a.real_shift));
 }
 
 // The new tokens of all sequences, a warp per (KV head, sequence), ahead of
@@ -232,34 +252,89 @@ __device__ void fp8_append_row(const Fp8Args& a, int b, int h, int L, int lane) 
 template <typename T, int D>
 __global__ void __launch_bounds__(32) fp8_append_kernel(const Fp8Args a) {
   griddep_wait();
-  const int b = blockIdx.y;
-  fp8_append_row<T, D>(a, b, blockIdx.x, clamp_ctx(a.context_lens, b, a.max_ctx, 1), threadIdx.x);
+  const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x, L = clamp_ctx(a.context_lens, b, a.max_ctx, 1);
+  NewRow<D> n;
+  fp8_load_new<T, D>(a, b, h, L, new_entry(a, b, L), lane, n);
+  fp8_store_new<D>(a, h, L, lane, n);
+}
+
+// Barrier operations and reads by shared-memory address: the producer's
+// per-stage loop has to stay small.
+__device__ __forceinline__ bool try_wait_at(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void expect_tx_at(uint32_t bar, uint32_t bytes) {
+  asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void tma_slice(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3, %2}], [%4], %5;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(bar), "l"(policy)
+      : "memory");
+}
+__device__ __forceinline__ int lds32(uint32_t a) {
+  int v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+
+// The bounded wait for a ring slot, out of line.  False: it ran out, or the
+// CTA has given up.
+__device__ __noinline__ bool slot_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int* err, uint32_t limit) {
+  for (uint32_t i = 0; i < limit && *gave_up == 0; ++i)
+    if (try_wait_at(bar, parity)) return true;
+  if (*gave_up == 0) {
+    atomicOr(err, CLOVE_FLAG_TIMEOUT);
+    *gave_up = 1;
+  }
+  return false;
 }
 
 // The producer warp (produce() of decode_common.cuh for this cache): walks
 // the CTA's range, posts each piece, appends the new token where the piece
-// ends its sequence, and streams the slices.  Table entries and scales are
-// loaded 32 slices at a time, half a group ahead of their use.
+// ends its sequence, and streams the slices.
+//
+// It must issue a stage every ~700 clocks beside the consumers, so what runs
+// once a stage is short, on one lane (a loop that leaves the instruction
+// cache costs over 1000 clocks here): the warp prepares 32 slices at a time
+// (table entries, copy rows, scales; loaded a group ahead), leaves the rows in
+// `rows` and the scales in the ring `scl`, and lane 0 issues their copies.
+// The scales of slice i of stage gs are at scl[(gs * sb + i) % kSclRing]: a
+// group is written when at most nstage stages are unconsumed, so nstage * sb +
+// 32 <= kSclRing entries are live.
 template <typename T, int D>
-__device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* tm_k, const CUtensorMap* tm_v, const SmemPtrs& sm,
-                            const SmemPlan& sp, float2* scl, int sb, const WalkStart& ws) {
+__device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* map, const SmemPtrs& sm, const SmemPlan& sp, float2* scl,
+                            int* rows, int sb, const WalkStart& ws) {
   constexpr int RPT = D >= 128 ? D / 128 : 1;  // rows of the copies' tensor map per token
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, sub_shift = a.real_shift - a.slice_shift;
   const int vs = a.block_size, H = a.num_kv_heads, Hq = H * a.group;
-  const uint32_t tile_bytes = (uint32_t)(vs * D);
+  const uint32_t slice_bytes = (uint32_t)(2 * vs * D);
   const uint32_t q_bytes = (uint32_t)(a.group * D * (int)sizeof(T));
   const uint64_t pol = policy_evict_first();
-  int slot = 0, uk = 0;
+  const uint32_t full = smem_u32(sm.full), empty = smem_u32(sm.empty), ring = smem_u32(sm.ring);
+  const uint32_t rows_at = smem_u32(rows), stage_bytes = (uint32_t)sp.stage_bytes;
+  int slot = 0, uk = 0, stage = 0;  // ring slot of the next stage, unit slot, stages issued
   uint32_t phase = 0, uphase = 0;
   bool aborted = false;
 
   // Lane i: the table entry of slice j0 + i of the piece (unchecked) ...
   auto entry = [&](const Unit& x, int j0) {
     const int j = j0 + lane;
-    return j < x.nblk ? __ldg(a.block_tables + (size_t)x.b * a.bt_stride + ((x.blk0 + j) >> a.sub_shift)) : 0;
+    return j < x.nblk ? __ldg(a.block_tables + (size_t)x.b * a.bt_stride + ((x.blk0 + j) >> sub_shift)) : 0;
   };
-  // ... and what it leads to: the copy's first row, the scales.  Entries
-  // outside the pool are flagged and replaced by block 0 (never followed).
+  // ... and what it leads to: the copy's first row, the scales (zero behind
+  // the piece).  Entries outside the pool are flagged and replaced by block 0
+  // (never followed).
   struct Slice {
     int row;
     float sk, sv;
@@ -273,22 +348,27 @@ __device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* tm_k, const CUt
         phys = 0;
       }
       const size_t tile = (size_t)phys * H + x.h;
-      s.row = ((int)tile * a.real_block + ((x.blk0 + j) & ((1 << a.sub_shift) - 1)) * vs) * RPT;
+      s.row = ((int)tile * a.real_block + ((x.blk0 + j) & ((1 << sub_shift) - 1)) * vs) * RPT;
       s.sk = __ldcg(a.scales + tile);
       s.sv = __ldcg(a.scales + (size_t)a.num_blocks * H + tile);
     }
     return s;
   };
 
-  const int alpha = a.seg_cost;
+  const int alpha = a.seg_cost, sb_shift = 31 - __clz(sb);
   int b = ws.b, h = ws.h, off = ws.off, npiece = 0;
-  long long pos = ws.lo;
+  int left = (int)(ws.hi - ws.lo);  // stream positions of the range still to walk
   int L = b >= 0 ? clamp_ctx(a.context_lens, b, a.max_ctx, a.append) : 0;
   int nb = L > 0 ? num_slices(a, L) : 0;
-  auto next_piece = [&](Unit& x, int& e0) -> bool {
-    while (b >= 0 && pos < ws.hi) {
-      const int len = nb + alpha;
-      const int span = (int)min((long long)(len - off), ws.hi - pos);
+  // What a piece needs from memory before its first copy, loaded while the
+  // piece before it still streams: the first slices and the new token.
+  Slice cur = {0, 0.f, 0.f};
+  NewRow<D> nr;
+  int e0 = 0, ne = 0;
+  // The next piece of the walk, with its first table entries under way.
+  auto claim = [&](Unit& x) -> bool {
+    while (b >= 0 && left > 0) {
+      const int len = nb + alpha, span = min(len - off, left);
       const int r0 = max(off, alpha), r1 = off + span;
       const bool piece = r1 > r0;
       if (piece) {
@@ -298,19 +378,22 @@ __device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* tm_k, const CUt
         x.L = L;
         x.blk0 = first_slice(a, L) + r0 - alpha;
         x.nblk = r1 - r0;
-        x.nstages = (x.nblk + sb - 1) / sb;
+        x.nstages = (x.nblk + sb - 1) >> sb_shift;
         x.complete = r0 == alpha && r1 == len;
         x.slot = npiece == 0 ? 0 : 1;
         x.last = r1 == len;
+        e0 = entry(x, 0);
+        if (a.append_here && x.last) ne = new_entry(a, b, L);
+        ++npiece;
       }
-      pos += span;
+      left -= span;
       off += span;
-      if (off == len && pos < ws.hi) {
+      if (off == len && left > 0) {
         off = 0;
         if (++h == H) {
           h = 0;
           do {
-            if (++b >= a.batch) {  // (cannot happen while pos < hi; bounds the walk regardless)
+            if (++b >= a.batch) {  // (cannot happen while positions are left; bounds the walk regardless)
               b = -1;
               break;
             }
@@ -319,102 +402,129 @@ __device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* tm_k, const CUt
           } while (L == 0);
         }
       }
-      if (piece) {
-        e0 = entry(x, 0);
-        ++npiece;
-        return true;
-      }
+      if (piece) return true;
     }
     return false;
   };
+  auto preload = [&](const Unit& x) {
+    cur = resolve(x, 0, e0);
+    if (a.append_here && x.last) fp8_load_new<T, D>(a, x.b, x.h, x.L, ne, lane, nr);
+  };
 
-  int e0 = 0;
+  // The walk starts behind an empty piece, so that there is one place in the
+  // code that claims and preloads.
   Unit x;
-  bool have = next_piece(x, e0);
-  bool first = true;
+  x.nblk = 0;
+  x.last = 0;
+  bool have = true, first = true;
   while (true) {
     int ok = 1;
-    if (lane == 0) {
-      if (*sm.misc || !mbar_wait_bounded(&sm.uempty[uk], uphase ^ 1, a.err, a.wait_limit)) {
-        ok = 0;
-        *sm.misc = 1;
-      } else if (!have) {
-        sm.slots[uk].valid = 0;
-        mbar_arrive(&sm.ufull[uk]);
-      } else {
-        sm.slots[uk].x = x;
-        sm.slots[uk].valid = 1;
-        mbar_arrive_expect_tx(&sm.ufull[uk], q_bytes);
-        const T* qsrc = static_cast<const T*>(a.q) + ((size_t)x.b * Hq + (size_t)x.h * a.group) * D;
-        bulk_load(sm.qbuf + uk * sp.q_stride, qsrc, q_bytes, &sm.ufull[uk]);
+    if (x.nblk > 0 || !have) {
+      if (lane == 0) {
+        if (!try_wait_at(smem_u32(&sm.uempty[uk]), uphase ^ 1) &&
+            !slot_wait(smem_u32(&sm.uempty[uk]), uphase ^ 1, sm.misc, a.err, a.wait_limit)) {
+          ok = 0;
+        } else if (!have) {
+          sm.slots[uk].valid = 0;
+          mbar_arrive(&sm.ufull[uk]);
+        } else {
+          sm.slots[uk].x = x;
+          sm.slots[uk].valid = 1;
+          mbar_arrive_expect_tx(&sm.ufull[uk], q_bytes);
+          const T* qsrc = static_cast<const T*>(a.q) + ((size_t)x.b * Hq + (size_t)x.h * a.group) * D;
+          bulk_load(sm.qbuf + uk * sp.q_stride, qsrc, q_bytes, &sm.ufull[uk]);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) {
+        aborted = true;
+        break;
+      }
+      if (!have) break;
+      if (++uk == kUnitRing) {
+        uk = 0;
+        uphase ^= 1;
       }
     }
-    ok = __shfl_sync(0xffffffffu, ok, 0);
+
+    if (a.append_here && x.last) {
+      fp8_store_new<D>(a, x.h, x.L, lane, nr);
+      // the scales loaded for the last block's slices are the old ones
+      const float sk = __shfl_sync(0xffffffffu, nr.old, 0), sv = __shfl_sync(0xffffffffu, nr.old, 16);
+      if (nr.phys >= 0 && lane < x.nblk && (x.blk0 + lane) >> sub_shift == (x.L - 1) >> a.real_shift) {
+        cur.sk = sk;
+        cur.sv = sv;
+      }
+    }
+    int e1 = x.nblk > 32 ? entry(x, 32) : 0;
+    Unit x2;
+    bool have2 = false;
+#pragma unroll 1
+    for (int j0 = 0; j0 == 0 || j0 < x.nblk; j0 += 32) {
+      const int n = min(32, x.nblk - j0);  // slices of this group
+      const bool final = j0 + 32 >= x.nblk;
+      rows[lane] = cur.row;
+      scl[(stage * sb + lane) & (kSclRing - 1)] = make_float2(cur.sk, cur.sv);
+      __syncwarp();
+      if (final) {
+        have2 = claim(x2);
+      } else {
+        cur = resolve(x, j0 + 32, e1);
+        if (j0 + 64 < x.nblk) e1 = entry(x, j0 + 64);
+      }
+      // lane 0 issues the group; before a piece's last stages the warp sees
+      // to the next piece's loads
+      const int nst = (n + sb - 1) >> sb_shift, cut = final ? (nst + 1) / 2 : nst;
+#pragma unroll 1
+      for (int part = 0; part < 2; ++part) {
+        const int s0 = part == 0 ? 0 : cut, s1 = part == 0 ? cut : nst;
+        if (lane == 0) {
+          int s = s0;
+          if (first && a.inject_stall && s < s1) {  // test hook: the CTA's first stage is never filled
+            ++s;
+            ++slot;
+          }
+          first = false;
+#pragma unroll 1
+          for (; s < s1; ++s) {
+            if (slot == a.nstage) {
+              slot = 0;
+              phase ^= 1;
+            }
+            if (!try_wait_at(empty + slot * 8, phase ^ 1) && !slot_wait(empty + slot * 8, phase ^ 1, sm.misc, a.err, a.wait_limit)) {
+              ok = 0;
+              break;
+            }
+            const int m = min(sb, n - s * sb);
+            const uint32_t bar = full + slot * 8;
+            expect_tx_at(bar, slice_bytes * (uint32_t)m);
+            uint32_t dst = ring + slot * stage_bytes, src = rows_at + s * sb * 4;
+#pragma unroll 1
+            for (int i = 0; i < m; ++i) {  // one copy per slice: its K tile, then its V tile
+              tma_slice(dst, map, bar, lds32(src), pol);
+              dst += slice_bytes;
+              src += 4;
+            }
+            ++slot;
+          }
+        }
+        __syncwarp();
+        if (part == 0 && final && have2) preload(x2);
+      }
+      stage += nst;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
+    }
     if (!ok) {
       aborted = true;
       break;
     }
-    if (!have) break;
-    if (++uk == kUnitRing) {
-      uk = 0;
-      uphase ^= 1;
-    }
-
-    if (a.append_here && x.last) fp8_append_row<T, D>(a, x.b, x.h, x.L, lane);
-    Slice cur = resolve(x, 0, e0), nxt = {0, 0.f, 0.f};
-    int e1 = x.nblk > 32 ? entry(x, 32) : 0;
-    int e2 = 0;
-    Unit x2;
-    bool have2 = false;
-    const int claim_at = min(x.nstages - 1, a.nstage / 2);
-    for (int s = 0; s < x.nstages; ++s) {
-      const int j0 = s * sb;
-      if ((j0 & 31) == 0 && j0 > 0) {
-        cur = nxt;
-        if (j0 + 32 < x.nblk) e1 = entry(x, j0 + 32);
-      }
-      if ((j0 & 31) == 16 && j0 + 16 < x.nblk) nxt = resolve(x, j0 + 16, e1);
-      const int n = min(sb, x.nblk - j0);
-      int ready = 1;
-      if (lane == 0 && (*sm.misc || !mbar_wait_bounded(&sm.empty[slot], phase ^ 1, a.err, a.wait_limit))) {
-        ready = 0;
-        *sm.misc = 1;
-      }
-      ready = __shfl_sync(0xffffffffu, ready, 0);
-      if (!ready) {
-        aborted = true;
-        break;
-      }
-      __syncwarp();
-      // the stage's scales, zero where it has no slice
-      const int from = (j0 + lane) & 31;
-      const float sk = __shfl_sync(0xffffffffu, cur.sk, from), sv = __shfl_sync(0xffffffffu, cur.sv, from);
-      if (lane < sb) scl[slot * kMaxSb + lane] = lane < n ? make_float2(sk, sv) : make_float2(0.f, 0.f);
-      __syncwarp();
-      const bool stall = a.inject_stall && first && s == 0;  // test hook: this stage is never filled
-      if (lane == 0 && !stall) mbar_arrive_expect_tx(&sm.full[slot], 2u * tile_bytes * (uint32_t)n);
-      __syncwarp();
-      const int row = __shfl_sync(0xffffffffu, cur.row, from);
-      if (lane < n && !stall) {
-        unsigned char* st = sm.ring + (size_t)slot * sp.stage_bytes;
-        tma_load_2d(st + lane * tile_bytes, tm_k, &sm.full[slot], 0, row, pol);
-        tma_load_2d(st + (sb + lane) * tile_bytes, tm_v, &sm.full[slot], 0, row, pol);
-      }
-      if (++slot == a.nstage) {
-        slot = 0;
-        phase ^= 1;
-      }
-      if (s == claim_at) have2 = next_piece(x2, e2);
-    }
-    if (aborted) break;
     have = have2;
     x = x2;
-    e0 = e2;
-    first = false;
   }
   if (aborted && lane == 0) {
     // drain: the last nstage stages and unit posts may still be in flight
-    int s = slot;
+    int s = slot;  // 1 .. nstage: the slot behind the last one issued
     uint32_t ph = phase;
     for (int k = 0; k < a.nstage; ++k) {
       if (--s < 0) {
@@ -437,10 +547,6 @@ __device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* tm_k, const CUt
   }
 }
 
-__device__ __forceinline__ void fence_proxy_async_smem() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
 // D(16x8, f32) += A(16x16, f16) * B(16x8, f16)
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -449,11 +555,36 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same from a zero accumulator.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Shared-memory reads by address (the compiler would take a generic pointer's
+// longer way).
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
-// Codes in the low / high 16 bits of w as an f16 pair.
-__device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return half2_bits(fp8_unpack2(w)); }
-__device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return half2_bits(fp8_unpack2(w >> 16)); }
+// Four codes -> two f16 pairs (low bytes first), exact.
+__device__ __forceinline__ void codes4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
 
 // x, y = hi + lo, each a pair of halves.
 __device__ __forceinline__ void split_halves(float x, float y, uint32_t& hi, uint32_t& lo) {
@@ -461,6 +592,25 @@ __device__ __forceinline__ void split_halves(float x, float y, uint32_t& hi, uin
   const float2 f = __half22float2(h);
   hi = half2_bits(h);
   lo = half2_bits(__floats2half2_rn(x - f.x, y - f.y));
+}
+
+// 16 bytes of elements, widened.
+template <typename T>
+__device__ __forceinline__ void unpack16(uint4 v, float* o) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      o[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      o[2 * i] = f.x;
+      o[2 * i + 1] = f.y;
+    } else {
+      o[2 * i] = __uint_as_float(w[i] << 16);
+      o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
 }
 
 // Byte offset of x within a stage's K (or V) region after the copy's swizzle.
@@ -479,47 +629,97 @@ __device__ __forceinline__ int k_chunk(int tq, int j) {
   return (j >> 1) * 8 + (tq & 1) + 4 * (tq >> 1) + 2 * (j & 1);
 }
 
+// The 8-byte V unit (8 dims of a 128-byte row) that lane row g reads as its
+// p-th: as for K, any assignment of dims to MMA columns will do.
+template <int D>
+__device__ __forceinline__ int v_unit(int g, int p) {
+  return D == 64 ? g : 2 * ((g & 1) + 2 * p + 4 * (g >> 2)) + ((g >> 1) & 1);
+}
+
+// 2^x; the hardware's, flushing results below 2^-126.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// tanh: up to kTanhNear the continued fraction x / (1 + x^2 / (3 + x^2 / (5 +
+// ..))) cut after the sixth level (off by less than 2^-27 there), beyond it
+// 1 - 2 / (1 + e^2x).  The library's version, unrolled over a pass, does not
+// fit the instruction cache beside the rest.
+constexpr float kTanhNear = 1.25f;
+__device__ __forceinline__ float tanh_near(float x) {
+  const float y = x * x;
+  return __fdividef(x * fmaf(y, fmaf(y, 21.f, 1260.f), 10395.f), fmaf(y, fmaf(y, y + 210.f, 4725.f), 10395.f));
+}
+__device__ __forceinline__ float tanh_far(float x) {
+  const float e = ex2(fabsf(x) * (2.f * kLog2e));
+  const float r = copysignf(1.f - __fdividef(2.f, 1.f + e), x);
+  return fabsf(x) > kTanhNear ? r : tanh_near(x);
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 // The power of two at or below x > 0 (within the range whose inverse is normal).
 __device__ __forceinline__ float floor_pow2(float x) {
   return __int_as_float(min(max(__float_as_int(x) & 0x7f800000, 1 << 23), 252 << 23));
 }
 __device__ __forceinline__ float inv_pow2(float x) { return __int_as_float((254 << 23) - __float_as_int(x)); }
 
-template <typename T, int D, int NCW>
-__global__ void __launch_bounds__((NCW + 1) * 32)
-    fp8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                      const Fp8Args a) {
-  constexpr int G = 8;
+// kExtra: scores may be capped, biased or kept (the plain variant has none of
+// that code: what a pass runs has to fit the instruction cache).
+template <typename T, int D, int NCW, bool kExtra>
+__global__ void __launch_bounds__((NCW + 1) * 32, 2)
+    fp8_decode_kernel(const __grid_constant__ CUtensorMap map, const Fp8Args a) {
+  static_assert(NCW == 3, "the hand-off sums three warps' states");
   constexpr bool kTwoHalves = sizeof(T) == 4;  // f32 queries need the low halves
   constexpr int KJ = D / 64;                   // 16-byte K chunks per lane and token
-  constexpr int VB = D >= 128 ? 16 : 8;        // V bytes per lane and token (per 128 dims)
-  constexpr int VH = D >= 128 ? D / 128 : 1;   // 128-dim halves
+  constexpr int VH = D >= 128 ? D / 128 : 1;   // 128-byte rows per token
+  constexpr int VP = D >= 128 ? 2 : 1;         // 8-byte V units per lane and row
   constexpr int NT = D / 8;                    // n-tiles of the value sum
-  const int vs = a.block_size, sb = a.stage_blocks, TT = sb * vs, group = a.group;
+  constexpr int S = state_stride(D);
+  constexpr int PT = D == 256 ? 32 : 64;       // tokens per pass
+  constexpr int NG = PT / 16, NE = PT / 8;     // MMA steps and 8-token tiles of a pass
+  constexpr int TT = stage_tokens(D);          // tokens per stage
+  const int vs = a.block_size, sb = a.stage_blocks, group = a.group;
 
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const SmemPlan sp = smem_plan(vs, D, 1, sb, a.nstage, NCW * group * state_stride(D) * (int)sizeof(float),
-                                group * D * (int)sizeof(T), a.nscr);
+  const SmemPlan sp = smem_plan(vs, D, 1, sb, a.nstage, (NCW - 1) * group * S * (int)sizeof(float),
+                                group * D * (int)sizeof(T), 1);
   const SmemPtrs sm = smem_ptrs(smem, sp, a.nstage);
-  float2* scl = reinterpret_cast<float2*>(reinterpret_cast<unsigned char*>(sm.scratch) + a.nscr * sp.scratch_bytes);
+  float2* scl = reinterpret_cast<float2*>(reinterpret_cast<unsigned char*>(sm.scratch) + sp.scratch_bytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    prefetch_tensor_map(&tm_k);
-    prefetch_tensor_map(&tm_v);
-  }
-  init_barriers(sm, a.nstage, NCW);
+  if (threadIdx.x == 0) prefetch_tensor_map(&map);
+  init_barriers<1, NCW - 1>(sm, a.nstage, NCW);
   __shared__ WalkStart walk;
   fp8_prologue<D>(a, &walk);
 
   if (warp == 0) {
-    fp8_produce<T, D>(a, &tm_k, &tm_v, sm, sp, scl, sb, walk);
+    fp8_produce<T, D>(a, &map, sm, sp, scl, reinterpret_cast<int*>(scl + kSclRing), sb, walk);
     return;
   }
 
   const int cw = warp - 1, g = lane >> 2, tq = lane & 3;
-  const int vshift = 31 - __clz(vs);
+  const int vshift = a.slice_shift;
+  // Read offsets within a pass: K rows g (+ 8 e), V rows 2 tq + (i & 1) (+ 8 n);
+  // the swizzle's row bits do not change with the multiples of 8 tokens.
+  uint32_t koff[KJ], voff[2][VH * VP];
+#pragma unroll
+  for (int j = 0; j < KJ; ++j) koff[j] = swz<D>((uint32_t)(g * D + k_chunk<D>(tq, j) * 16));
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int k = 0; k < VH * VP; ++k)
+      voff[i][k] = swz<D>((uint32_t)((2 * tq + i) * D + (k / VP) * 128 + v_unit<D>(g, k % VP) * 8));
+  // A stage is slice after slice, K tile then V tile: the K rows of token tok
+  // (a multiple of 8) from the stage's start, its V rows one tile further.
+  auto tile_at = [&](int tok) { return (uint32_t)((tok + (tok & -vs)) * D); };
   int gbase = 0, uk = 0, n_done = 0;
   uint32_t uphase = 0;
   UnitSlot us;
@@ -528,209 +728,236 @@ __global__ void __launch_bounds__((NCW + 1) * 32)
     const Unit x = us.x;
     // Query fragments: row g scaled by a power of two that puts its largest
     // element in [2^13, 2^14), undone in the score's factor.
-    uint32_t qa[KJ * 4][kTwoHalves ? 4 : 2];
-    float zf;  // score = dot * K scale * zf
-    {
-      const T* qrow = reinterpret_cast<const T*>(sm.qbuf + uk * sp.q_stride) + g * D;
+    uint32_t qh[KJ * 4][2], ql[kTwoHalves ? KJ * 4 : 1][2];
+    float zf[2], slope[2];  // of queries 2 tq and 2 tq + 1: score = dot * K scale * zf, bias per token
+    // stage gs belongs to warp gs % NCW (nstage is a multiple of NCW)
+    const int j_first = ((cw - gbase) % NCW + NCW) % NCW;
+    const bool mine = j_first < x.nstages;
+    if (mine) {
+      const uint32_t qaddr = smem_u32(sm.qbuf + uk * sp.q_stride) + g * D * (int)sizeof(T);
+      float q[KJ * 16];
       float amax = 0.f;
-      if (g < group) {
 #pragma unroll
-        for (int j = 0; j < KJ; ++j)
+      for (int j = 0; j < KJ; ++j)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(Elem<T>::to_f(qrow[k_chunk<D>(tq, j) * 16 + i])));
-      }
+        for (int i = 0; i < 16; i += 16 / (int)sizeof(T)) {
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (g < group) w = lds128(qaddr + (k_chunk<D>(tq, j) * 16 + i) * (int)sizeof(T));
+          unpack16<T>(w, q + j * 16 + i);
+        }
+#pragma unroll
+      for (int i = 0; i < KJ * 16; ++i) amax = fmaxf(amax, fabsf(q[i]));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      const float unit = floor_pow2(amax);
-      const int e = min((__float_as_int(unit) >> 23) - 127 - 13, 126);  // divide by 2^e
+      const int e = (__float_as_int(floor_pow2(amax)) >> 23) - 127 - 13;  // divide by 2^e
       const float up = __int_as_float((127 - max(e, -127)) << 23);
-      zf = a.scale * __int_as_float((127 + max(e, -126)) << 23);
-      if (e < -126) zf *= 0.5f;
+      float f = a.scale * __int_as_float((127 + max(e, -126)) << 23);
+      if (e < -126) f *= 0.5f;
+      f = kExtra && a.softcap > 0.f ? f / a.softcap : f * kLog2e;
+      const float s = kExtra && a.slopes != nullptr && g < group ? __ldg(a.slopes + x.h * group + g) * kLog2e : 0.f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        zf[c] = __shfl_sync(0xffffffffu, f, (2 * tq + c) * 4);
+        slope[c] = __shfl_sync(0xffffffffu, s, (2 * tq + c) * 4);
+      }
 #pragma unroll
       for (int j = 0; j < KJ; ++j)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          float f[4] = {0.f, 0.f, 0.f, 0.f};
-          if (g < group) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = Elem<T>::to_f(qrow[k_chunk<D>(tq, j) * 16 + w * 4 + i]) * up;
-          }
-          uint32_t lo0, lo1;
-          split_halves(f[0], f[1], qa[j * 4 + w][0], lo0);
-          split_halves(f[2], f[3], qa[j * 4 + w][1], lo1);
+          const float* f4 = q + j * 16 + w * 4;
+          uint32_t lo[2];
+          split_halves(f4[0] * up, f4[1] * up, qh[j * 4 + w][0], lo[0]);
+          split_halves(f4[2] * up, f4[3] * up, qh[j * 4 + w][1], lo[1]);
           if constexpr (kTwoHalves) {
-            qa[j * 4 + w][2] = lo0;
-            qa[j * 4 + w][3] = lo1;
+            ql[j * 4 + w][0] = lo[0];
+            ql[j * 4 + w][1] = lo[1];
           }
         }
     }
-    const int hq = x.h * group + g;
-    const float cap = a.softcap;
-    zf = cap > 0.f ? zf / cap : zf * kLog2e;
-    const float slope = a.slopes != nullptr && g < group ? __ldg(a.slopes + hq) * kLog2e : 0.f;
+    const float cap = a.softcap * kLog2e;
     const int t_first = a.window > 0 ? max(0, x.L - a.window) : 0;  // first token attended to
-    float* zrow = a.z != nullptr && g < group
-                      ? a.z + ((size_t)x.b * a.num_kv_heads * group + hq) * a.z_stride
+    float* zrow = kExtra && a.z != nullptr
+                      ? a.z + ((size_t)(x.b * a.num_kv_heads + x.h) * group + 2 * tq) * a.z_stride
                       : nullptr;
 
-    float m = -INFINITY, l = 0.f, vref = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, vref = 0.f;
     float o[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = 0.f;
 
     bool aborted = false;
-    const int ncw = a.ncw;
-    // Stage gs belongs to warp gs % ncw; nstage is a multiple of ncw.
-    for (int j = cw < ncw ? ((cw - gbase) % ncw + ncw) % ncw : x.nstages; j < x.nstages; j += ncw) {
+    for (int j = j_first; j < x.nstages; j += NCW) {
       const int gs = gbase + j, slot = gs % a.nstage;
       if (!wait_or_abort(a, sm, &sm.full[slot], (uint32_t)(gs / a.nstage) & 1u)) {
         aborted = true;
         break;
       }
-      unsigned char* kst = sm.ring + (size_t)slot * sp.stage_bytes;
-      unsigned char* vst = kst + sb * sp.tile_stride;
-      const float2* sc = scl + slot * kMaxSb;
+      const uint32_t kbase = smem_u32(sm.ring + (size_t)slot * sp.stage_bytes);
+      const uint32_t vbase = kbase + sp.tile_stride, sbase = smem_u32(scl);
+      const int s_first = gs * sb;                // scale ring index of the stage's first slice
       const int t_base = (x.blk0 + j * sb) * vs;  // token of the stage's first row
       const int hi = min(TT, min((x.blk0 + x.nblk) * vs, x.L) - t_base), lo = max(0, t_first - t_base);
       const bool ragged = lo > 0 || hi < TT;
       if (ragged) {
         // Rows outside [lo, hi) may hold NaN codes; their weights are 0, but
         // 0 * NaN is NaN, so clear those V rows.
+        unsigned char* vst = sm.ring + (size_t)slot * sp.stage_bytes + sp.tile_stride;
         for (int i = lane; i < TT * (D / 16); i += 32) {
           const int tok = i / (D / 16);
-          if (tok < lo || tok >= hi) *reinterpret_cast<uint4*>(vst + swz<D>(i * 16)) = make_uint4(0, 0, 0, 0);
+          if (tok < lo || tok >= hi) *reinterpret_cast<uint4*>(vst + (tok & -vs) * D + swz<D>(i * 16)) = make_uint4(0, 0, 0, 0);
         }
         __syncwarp();
       }
-      for (int p0 = 0; p0 < hi; p0 += 32) {
-        // ---- scores of 32 tokens: four tiles of 8 ----
-        float z[4][2], wv[4];
+#pragma unroll 1
+      for (int p0 = 0; p0 < (TT == PT ? 1 : hi); p0 += PT) {
+        // ---- scores: tile e is tokens p0 + 8 e + g, queries 2 tq + c ----
+        float z[NE][2], wv[NE];
         float vmax = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint4 kw[KJ];
+        for (int k = 0; k < NG; ++k) {
+          uint4 kw[2][KJ];
 #pragma unroll
-          for (int c = 0; c < KJ; ++c)
-            kw[c] = *reinterpret_cast<const uint4*>(
-                kst + swz<D>((uint32_t)((p0 + 8 * e + g) * D + k_chunk<D>(tq, c) * 16)));
-          float s[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int c = 0; c < KJ; ++c) kw[r][c] = lds128(kbase + koff[c] + tile_at(p0 + 16 * k + 8 * r));
+          float s[4];
 #pragma unroll
           for (int c = 0; c < KJ; ++c) {
-            const uint32_t w[4] = {kw[c].x, kw[c].y, kw[c].z, kw[c].w};
+            const uint32_t w0[4] = {kw[0][c].x, kw[0][c].y, kw[0][c].z, kw[0][c].w};
+            const uint32_t w1[4] = {kw[1][c].x, kw[1][c].y, kw[1][c].z, kw[1][c].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint32_t* q = qa[c * 4 + i];
-              if constexpr (kTwoHalves)
-                mma_f16(s, q[0], q[2], q[1], q[3], codes_lo(w[i]), codes_hi(w[i]));
+              uint32_t a0, a1, a2, a3;
+              codes4(w0[i], a0, a2);
+              codes4(w1[i], a1, a3);
+              if (c == 0 && i == 0)
+                mma_f16_first(s, a0, a1, a2, a3, qh[0][0], qh[0][1]);
               else
-                mma_f16(s, q[0], 0u, q[1], 0u, codes_lo(w[i]), codes_hi(w[i]));
+                mma_f16(s, a0, a1, a2, a3, qh[c * 4 + i][0], qh[c * 4 + i][1]);
+              if constexpr (kTwoHalves) mma_f16(s, a0, a1, a2, a3, ql[c * 4 + i][0], ql[c * 4 + i][1]);
             }
           }
-          const float2 f = sc[(p0 + 8 * e) >> vshift];
-          const float kf = f.x * zf;
-          wv[e] = f.y;
-          vmax = fmaxf(vmax, f.y);
-          z[e][0] = (kTwoHalves ? s[0] + s[2] : s[0]) * kf;
-          z[e][1] = (kTwoHalves ? s[1] + s[3] : s[1]) * kf;
-        }
-        if (cap > 0.f) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            z[e][0] = tanhf(z[e][0]) * (cap * kLog2e);
-            z[e][1] = tanhf(z[e][1]) * (cap * kLog2e);
+          for (int r = 0; r < 2; ++r) {
+            const int e = 2 * k + r;
+            const uint2 f = lds64(sbase + ((s_first + ((p0 + 8 * e) >> vshift)) & (kSclRing - 1)) * 8);
+            wv[e] = __uint_as_float(f.y);
+            vmax = fmaxf(vmax, wv[e]);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) z[e][c] = s[2 * r + c] * (__uint_as_float(f.x) * zf[c]);
           }
         }
-        if (a.slopes != nullptr) {
-          const int back = t_base + p0 + 2 * tq - (x.L - 1);
+        if constexpr (kExtra) {
+          if (cap > 0.f) {
+            float most = 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            z[e][0] = fmaf(slope, (float)(back + 8 * e), z[e][0]);
-            z[e][1] = fmaf(slope, (float)(back + 8 * e + 1), z[e][1]);
+            for (int e = 0; e < NE; ++e) most = fmaxf(most, fmaxf(fabsf(z[e][0]), fabsf(z[e][1])));
+            if (__any_sync(0xffffffffu, most > kTanhNear)) {
+#pragma unroll
+              for (int e = 0; e < NE; ++e)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) z[e][c] = tanh_far(z[e][c]) * cap;
+            } else {
+#pragma unroll
+              for (int e = 0; e < NE; ++e)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) z[e][c] = tanh_near(z[e][c]) * cap;
+            }
           }
-        }
-        if (zrow != nullptr) {
+          if (a.slopes != nullptr) {
+            const float back = (float)(t_base + p0 + g - (x.L - 1));  // exact below 2^24
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (p0 + 8 * e + 2 * tq < hi)
-              *reinterpret_cast<float2*>(zrow + t_base + p0 + 8 * e + 2 * tq) = make_float2(z[e][0], z[e][1]);
+            for (int e = 0; e < NE; ++e)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) z[e][c] = fmaf(slope[c], back + (float)(8 * e), z[e][c]);
+          }
+          if (zrow != nullptr) {
+            const int left = hi - p0 - g;  // tokens of this lane's column
+            float* zt = zrow + t_base + p0 + g;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              if (2 * tq + c < group) {
+#pragma unroll
+                for (int e = 0; e < NE; ++e)
+                  if (8 * e < left) zt[8 * e] = z[e][c];
+              }
+              zt += a.z_stride;
+            }
+          }
         }
         if (ragged) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int tok = p0 + 8 * e + 2 * tq + c;
-              if (tok < lo || tok >= hi) z[e][c] = -INFINITY;
-            }
+          for (int e = 0; e < NE; ++e) {
+            const int tok = p0 + 8 * e + g;
+            if (tok < lo || tok >= hi) z[e][0] = z[e][1] = -INFINITY;
+          }
         }
-        // ---- online softmax of row g ----
-        float mx = z[0][0];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fmaxf(z[e][0], z[e][1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m, mx);
-        const float ms = mn == -INFINITY ? 0.f : mn - 14.f;
-        const float corr = m == -INFINITY ? 0.f : exp2f(m - mn);
-        m = mn;
+        // ---- online softmax of queries 2 tq and 2 tq + 1 ----
         const float vnew = fmaxf(vref, floor_pow2(vmax)), vinv = inv_pow2(vnew);
-        const float oc = corr * (vref * vinv);
-        vref = vnew;
-        float ps = 0.f;
-        uint32_t ph[4], pl[4];
+        float corr[2], ms[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p0e = exp2f(z[e][0] - ms), p1e = exp2f(z[e][1] - ms);
-          ps += p0e + p1e;
-          const float f = wv[e] * vinv;
-          split_halves(p0e * f, p1e * f, ph[e], pl[e]);
+        for (int c = 0; c < 2; ++c) {
+          float mx = z[0][c];
+#pragma unroll
+          for (int e = 1; e < NE; ++e) mx = fmaxf(mx, z[e][c]);
+#pragma unroll
+          for (int s = 4; s < 32; s <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
+          const float mn = fmaxf(m[c], mx);
+          ms[c] = mn == -INFINITY ? 0.f : mn - 14.f;
+          corr[c] = m[c] == -INFINITY ? 0.f : ex2(m[c] - mn);
+          m[c] = mn;
+          l[c] *= corr[c];
         }
-        l = fmaf(l, corr, ps);
-        // ---- value sum: two 16-token steps ----
-        // Lane column g of an n-tile is dims g * VB + byte (of each 128-dim half).
+        // the P operand: high halves in rows 0..7, low halves in rows 8..15
+        uint32_t pa[NG][4];
 #pragma unroll
-        for (int half = 0; half < VH; ++half) {
-          uint32_t vw[2][4][VB / 4];
+        for (int e = 0; e < NE; ++e) {
+          const float p0e = ex2(z[e][0] - ms[0]), p1e = ex2(z[e][1] - ms[1]), f = wv[e] * vinv;
+          l[0] += p0e;
+          l[1] += p1e;
+          uint32_t ph, pl;
+          split_halves(p0e * f, p1e * f, ph, pl);
+          pa[e >> 1][2 * (e & 1)] = transpose8x8(ph);
+          pa[e >> 1][2 * (e & 1) + 1] = transpose8x8(pl);
+        }
+        // the value sum's rows are queries g: their correction is held by lanes tq = g / 2
+        const float c0 = __shfl_sync(0xffffffffu, corr[0], g >> 1), c1 = __shfl_sync(0xffffffffu, corr[1], g >> 1);
+        const float oc = (g & 1 ? c1 : c0) * (vref * vinv);
+        vref = vnew;
+        // ---- value sum ----
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
+        for (int u = 0; u < VH * VP; ++u) {
+          uint2 vw[NG][4];  // tokens 16 k + 2 tq + {0, 1, 8, 9}, 8 dims each
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int tok = p0 + 16 * k + 2 * tq + (i & 1) + 8 * (i >> 1);
-              const unsigned char* src = vst + swz<D>((uint32_t)(tok * D + half * 128 + g * VB));
-              if constexpr (VB == 16) {
-                const uint4 w = *reinterpret_cast<const uint4*>(src);
-                vw[k][i][0] = w.x;
-                vw[k][i][1] = w.y;
-                vw[k][i][2] = w.z;
-                vw[k][i][3] = w.w;
-              } else {
-                const uint2 w = *reinterpret_cast<const uint2*>(src);
-                vw[k][i][0] = w.x;
-                vw[k][i][1] = w.y;
+          for (int k = 0; k < NG; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              vw[k][i] = lds64(vbase + voff[i & 1][u] + tile_at(p0 + 16 * k + 8 * (i >> 1)));
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            float d[4][4];
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+              const uint32_t t0 = w ? vw[k][0].y : vw[k][0].x, t1 = w ? vw[k][1].y : vw[k][1].x;
+              const uint32_t t2 = w ? vw[k][2].y : vw[k][2].x, t3 = w ? vw[k][3].y : vw[k][3].x;
+              uint32_t b0[4], b1[4];  // token pairs of dims 0..3
+              codes4(__byte_perm(t0, t1, 0x5140), b0[0], b0[1]);
+              codes4(__byte_perm(t0, t1, 0x7362), b0[2], b0[3]);
+              codes4(__byte_perm(t2, t3, 0x5140), b1[0], b1[1]);
+              codes4(__byte_perm(t2, t3, 0x7362), b1[2], b1[3]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (k == 0)
+                  mma_f16_first(d[i], pa[0][0], pa[0][1], pa[0][2], pa[0][3], b0[i], b1[i]);
+                else
+                  mma_f16(d[i], pa[k][0], pa[k][1], pa[k][2], pa[k][3], b0[i], b1[i]);
               }
             }
 #pragma unroll
-          for (int w = 0; w < VB / 4; ++w) {
-            uint32_t b0[2][2], b1[2][2];  // [step][dims 0,1 | 2,3]: token pairs of two dims
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              b0[k][0] = __byte_perm(vw[k][0][w], vw[k][1][w], 0x5140);
-              b0[k][1] = __byte_perm(vw[k][0][w], vw[k][1][w], 0x7362);
-              b1[k][0] = __byte_perm(vw[k][2][w], vw[k][3][w], 0x5140);
-              b1[k][1] = __byte_perm(vw[k][2][w], vw[k][3][w], 0x7362);
-            }
-#pragma unroll
             for (int i = 0; i < 4; ++i) {
-              float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const uint32_t x0 = i & 1 ? codes_hi(b0[k][i >> 1]) : codes_lo(b0[k][i >> 1]);
-                const uint32_t x1 = i & 1 ? codes_hi(b1[k][i >> 1]) : codes_lo(b1[k][i >> 1]);
-                mma_f16(d, ph[2 * k], pl[2 * k], ph[2 * k + 1], pl[2 * k + 1], x0, x1);
-              }
-              float* on = o[half * 16 + w * 4 + i];
-              on[0] = fmaf(on[0], oc, d[0] + d[2]);
-              on[1] = fmaf(on[1], oc, d[1] + d[3]);
+              float* on = o[u * 8 + w * 4 + i];
+              on[0] = fmaf(on[0], oc, d[i][0] + d[i][2]);
+              on[1] = fmaf(on[1], oc, d[i][1] + d[i][3]);
             }
           }
         }
@@ -742,29 +969,108 @@ __global__ void __launch_bounds__((NCW + 1) * 32)
     if (aborted) return;  // the abort flag is up; every other warp leaves at its next wait
     gbase += x.nstages;
 
-    // ---- publish (acc, m - 14, l) of the group's rows, hand off ----
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    const int sbuf = n_done % a.nscr;
-    if (!wait_or_abort(a, sm, &sm.scr_empty[sbuf], ((uint32_t)(n_done / a.nscr) & 1u) ^ 1u)) return;
-    float* scr = sm.scratch + sbuf * sm.scratch_floats + (size_t)(cw * group + g) * state_stride(D);
-    if (g < group) {
-      // thread (g, tq) holds columns 2 tq and 2 tq + 1 of every n-tile
+    // ---- hand-off: the last warp to finish a piece merges the others' states
+    // (acc, m - 14, l), left in scratch, with its own, still in registers ----
 #pragma unroll
-      for (int half = 0; half < VH; ++half)
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int s = 4; s < 32; s <<= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], s);
+    const uint32_t par = (uint32_t)n_done & 1u;
+    if (!wait_or_abort(a, sm, &sm.scr_empty[0], par ^ 1u)) return;
+    int order = 0;
+    if (lane == 0) {
+      order = atomicAdd(&sm.arrive[0], 1);
+      mbar_arrive(&sm.uempty[uk]);  // this warp no longer reads the unit's slot
+    }
+    order = __shfl_sync(0xffffffffu, order, 0);
+    if (order < NCW - 1) {
+      float* scr = sm.scratch + (size_t)order * group * S;
+      if (g < group && mine) {
+        // thread (g, tq) holds columns 2 tq and 2 tq + 1 of every n-tile
+        float* row = scr + (size_t)g * S;
+#pragma unroll
+        for (int u = 0; u < VH * VP; ++u)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; i += 4)
+              *reinterpret_cast<float4*>(row + (u / VP) * 128 + v_unit<D>(2 * tq + c, u % VP) * 8 + i) =
+                  make_float4(o[u * 8 + i][c] * vref, o[u * 8 + i + 1][c] * vref, o[u * 8 + i + 2][c] * vref,
+                              o[u * 8 + i + 3][c] * vref);
+      }
+      if (g == 0) {
 #pragma unroll
         for (int c = 0; c < 2; ++c)
+          if (2 * tq + c < group) {
+            scr[(size_t)(2 * tq + c) * S + D] = m[c] - 14.f;
+            scr[(size_t)(2 * tq + c) * S + D + 1] = l[c];
+            scr[(size_t)(2 * tq + c) * S + D + 2] = (float)cw;
+          }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.scr_empty[1]);  // [1]: the others' states are in scratch
+    } else {
+      if (!wait_or_abort(a, sm, &sm.scr_empty[1], par)) return;
+      // row g: this warp's m and l from the lanes that hold them, the others' from scratch
+      const float m0 = __shfl_sync(0xffffffffu, m[0], g >> 1), m1 = __shfl_sync(0xffffffffu, m[1], g >> 1);
+      const float l0 = __shfl_sync(0xffffffffu, l[0], g >> 1), l1 = __shfl_sync(0xffffffffu, l[1], g >> 1);
+      if (g < group) {
+        // Which warp comes last differs from run to run, the sums must not:
+        // they are (warp 0 + warp 1) + warp 2, A and B being the others' states
+        // in the order of their warps.
+        const float* A = sm.scratch + (size_t)g * S;
+        const float* B = A + (size_t)group * S;
+        if (A[D + 2] > B[D + 2]) {
+          const float* swap = A;
+          A = B;
+          B = swap;
+        }
+        const bool own_last = cw == NCW - 1;
+        // fo xo + fa xa + fb xb, each product rounded (a contracted one would tell who came last)
+        auto add = [&](float wo, float xo, float wa, float xa, float wb, float xb) {
+          const float po = __fmul_rn(wo, xo), pb = __fmul_rn(wb, xb);
+          return __fadd_rn(__fadd_rn(own_last ? pb : po, __fmul_rn(wa, xa)), own_last ? po : pb);
+        };
+        const float mo = (g & 1 ? m1 : m0) - 14.f, M = fmaxf(mo, fmaxf(A[D], B[D]));
+        const float fo = mo == -INFINITY ? 0.f : ex2(mo - M);
+        const float fa = A[D] == -INFINITY ? 0.f : ex2(A[D] - M), fb = B[D] == -INFINITY ? 0.f : ex2(B[D] - M);
+        const float L = add(fo, g & 1 ? l1 : l0, fa, A[D + 1], fb, B[D + 1]);
+        const float inv = 1.f / L, norm = x.complete ? inv : 1.f;
+        const int Hq = a.num_kv_heads * group, hq = x.h * group + g;
+        float* dst = x.complete ? a.out + ((size_t)x.b * Hq + hq) * D
+                                : a.partials + (((size_t)blockIdx.x * 2 + x.slot) * group + g) * S;
 #pragma unroll
-          for (int i = 0; i < VB; i += 4)
-            *reinterpret_cast<float4*>(scr + half * 128 + (2 * tq + c) * VB + i) =
-                make_float4(o[half * 16 + i][c] * vref, o[half * 16 + i + 1][c] * vref, o[half * 16 + i + 2][c] * vref,
-                            o[half * 16 + i + 3][c] * vref);
-      if (tq == 0) {
-        scr[D] = m - 14.f;
-        scr[D + 1] = l;
+        for (int u = 0; u < VH * VP; ++u)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+              const int d = (u / VP) * 128 + v_unit<D>(2 * tq + c, u % VP) * 8 + i;
+              // (a warp without a stage of the piece leaves no acc)
+              float4 va = make_float4(0.f, 0.f, 0.f, 0.f), vb = va;
+              if (fa > 0.f) va = *reinterpret_cast<const float4*>(A + d);
+              if (fb > 0.f) vb = *reinterpret_cast<const float4*>(B + d);
+              *reinterpret_cast<float4*>(dst + d) =
+                  make_float4(add(fo, __fmul_rn(o[u * 8 + i][c], vref), fa, va.x, fb, vb.x) * norm,
+                              add(fo, __fmul_rn(o[u * 8 + i + 1][c], vref), fa, va.y, fb, vb.y) * norm,
+                              add(fo, __fmul_rn(o[u * 8 + i + 2][c], vref), fa, va.z, fb, vb.z) * norm,
+                              add(fo, __fmul_rn(o[u * 8 + i + 3][c], vref), fa, va.w, fb, vb.w) * norm);
+            }
+        if (tq == 0) {
+          if (!x.complete) {
+            dst[D] = M;
+            dst[D + 1] = L;
+          } else if (kExtra && a.row_state != nullptr) {
+            a.row_state[(size_t)x.b * Hq + hq] = make_float2(M, inv);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) {
+        sm.arrive[0] = 0;
+        mbar_arrive(&sm.scr_empty[0]);
       }
     }
-    hand_off<D, G, NCW>(a, sm, us, sbuf, uk, lane);
     ++n_done;
     if (++uk == kUnitRing) {
       uk = 0;
@@ -807,8 +1113,9 @@ __global__ void __launch_bounds__(kMassThreads) fp8_mass_kernel(const Fp8Args a)
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-constexpr int kFp8Warps = 4;
+constexpr int kFp8Warps = 3;
 constexpr int kFp8Ring = 96 * 1024;
+constexpr int kFp8Smem = 227 * 1024 / 2 - 1024;  // of each of two CTAs on an SM
 
 // Stream positions charged per segment for a piece's fixed cost: 40 KB worth
 // of slices, as for the other decodes.
@@ -846,35 +1153,30 @@ size_t fp8_decode_workspace(const clove_fp8_pool& pool, int batch, int num_q_hea
   return fp8_layout(pool, batch, num_q_heads, max_ctx, accumulate).total;
 }
 
-// One plane of codes as rows of 128 bytes (64 for head_dim 64), a box being
-// one slice of a tile.
-static int fp8_plane_map(CUtensorMap* map, void* base, const clove_fp8_pool& pool, int slice) {
+// The codes as rows of 128 bytes (64 for head_dim 64) in two planes, a box
+// being the K and V parts of one slice.
+int fp8_encode_map(clove_fp8_pool& pool) {
   auto fn = tensor_map_encoder();
   if (!fn) {
     set_last_error("cuTensorMapEncodeTiled unavailable from the driver");
     return CLOVE_ERR_CUDA;
   }
+  const int slice = std::min(pool.block_size, stage_tokens(pool.head_dim));
   const cuuint32_t inner = pool.head_dim >= 128 ? 128 : 64, rpt = pool.head_dim / inner;
-  cuuint64_t dims[2] = {inner, (cuuint64_t)pool.plane_bytes / inner};
-  cuuint64_t strides[1] = {inner};
-  cuuint32_t box[2] = {inner, (cuuint32_t)slice * rpt};
-  cuuint32_t estr[2] = {1, 1};
-  const CUresult r =
-      fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-         inner == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  cuuint64_t dims[3] = {inner, (cuuint64_t)pool.plane_bytes / inner, 2};
+  cuuint64_t strides[2] = {inner, (cuuint64_t)pool.plane_bytes};
+  cuuint32_t box[3] = {inner, (cuuint32_t)slice * rpt, 2};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(&pool.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, pool.codes, dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        inner == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_last_error("cuTensorMapEncodeTiled failed (%d) for head_dim %d block_size %d", (int)r, pool.head_dim,
                    pool.block_size);
     return CLOVE_ERR_CUDA;
   }
   return CLOVE_OK;
-}
-
-int fp8_encode_maps(clove_fp8_pool& pool) {
-  const int slice = std::min(pool.block_size, kSlice);
-  const int rc = fp8_plane_map(&pool.tm_k, pool.codes, pool, slice);
-  return rc ? rc : fp8_plane_map(&pool.tm_v, pool.codes + pool.plane_bytes, pool, slice);
 }
 
 template <typename K, typename... A>
@@ -898,12 +1200,12 @@ struct Fp8Cfg {
   int nstage, smem, ctas;
 };
 
-template <typename T, int D>
-static int fp8_cfg(const clove_fp8_pool& pool, int slice, int group, int nscr, Fp8Cfg* out) {
+template <typename T, int D, bool kExtra>
+static int fp8_cfg(const clove_fp8_pool& pool, int slice, int group, Fp8Cfg* out) {
   static std::mutex mu;
   static std::unordered_map<long long, Fp8Cfg> cache;
   static std::unordered_map<int, int> attr;  // device -> shared memory the kernel may use there
-  auto kern = fp8_decode_kernel<T, D, kFp8Warps>;
+  auto kern = fp8_decode_kernel<T, D, kFp8Warps, kExtra>;
   const long long key = ((long long)pool.device << 32) | ((long long)slice << 8) | group;
   std::lock_guard<std::mutex> lk(mu);
   auto it = cache.find(key);
@@ -916,12 +1218,17 @@ static int fp8_cfg(const clove_fp8_pool& pool, int slice, int group, int nscr, F
     return v ? std::atoi(v) : 0;
   }();
   const int ring = ring_kb > 0 ? ring_kb * 1024 : kFp8Ring;
-  const int sb = stage_tokens<D>() / slice;
-  const int scratch = kFp8Warps * group * state_stride(D) * 4, qb = group * D * (int)sizeof(T);
+  const int sb = stage_tokens(D) / slice;
+  const int scratch = (kFp8Warps - 1) * group * state_stride(D) * 4, qb = group * D * (int)sizeof(T);
   Fp8Cfg c;
-  const int stage = smem_plan(slice, D, 1, sb, 1, scratch, qb, nscr).stage_bytes;
+  const int stage = smem_plan(slice, D, 1, sb, 1, scratch, qb, 1).stage_bytes;
+  auto bytes = [&](int n) {
+    return smem_plan(slice, D, 1, sb, n, scratch, qb, 1).total + kSclRing * (int)sizeof(float2) + 32 * (int)sizeof(int) + 1024;
+  };
+  // as deep a ring as two CTAs on an SM leave room for
   c.nstage = std::max(1, ring / stage / kFp8Warps) * kFp8Warps;
-  c.smem = smem_plan(slice, D, 1, sb, c.nstage, scratch, qb, nscr).total + c.nstage * kMaxSb * (int)sizeof(float2) + 1024;
+  while (c.nstage > kFp8Warps && (bytes(c.nstage) > kFp8Smem || c.nstage * sb + 32 > kSclRing)) c.nstage -= kFp8Warps;
+  c.smem = bytes(c.nstage);
   if (c.smem > attr[pool.device]) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, c.smem);
     if (e != cudaSuccess) return fp8_launch_status("cudaFuncSetAttribute", e);
@@ -939,12 +1246,11 @@ static int fp8_cfg(const clove_fp8_pool& pool, int slice, int group, int nscr, F
   return CLOVE_OK;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kExtra>
 static int run_fp8(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) {
-  a.stage_blocks = stage_tokens<D>() / a.block_size;
-  a.nscr = a.group > 4 ? 2 : 1;
+  a.stage_blocks = stage_tokens(D) / a.block_size;
   Fp8Cfg c;
-  int rc = fp8_cfg<T, D>(pool, a.block_size, a.group, a.nscr, &c);
+  int rc = fp8_cfg<T, D, kExtra>(pool, a.block_size, a.group, &c);
   if (rc) return rc;
   a.nstage = c.nstage;
   a.ncw = kFp8Warps;
@@ -960,8 +1266,8 @@ static int run_fp8(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) 
     count_launches(1);
   }
   rc = fp8_launch_status("fp8_decode launch",
-                         launch_chained(fp8_decode_kernel<T, D, kFp8Warps>, dim3(a.num_ctas), (kFp8Warps + 1) * 32,
-                                        c.smem, stream, pool.tm_k, pool.tm_v, a));
+                         launch_chained(fp8_decode_kernel<T, D, kFp8Warps, kExtra>, dim3(a.num_ctas), (kFp8Warps + 1) * 32,
+                                        c.smem, stream, pool.map, a));
   if (rc) return rc;
   count_launches(1);
   if (!a.direct) {
@@ -980,19 +1286,25 @@ static int run_fp8(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) 
   return CLOVE_OK;
 }
 
+template <typename T, int D>
+static int run_fp8_scores(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) {
+  const bool extra = a.softcap > 0.f || a.slopes != nullptr || a.z != nullptr;
+  return extra ? run_fp8<T, D, true>(pool, a, stream) : run_fp8<T, D, false>(pool, a, stream);
+}
+
 template <typename T>
 static int run_fp8_dim(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) {
   switch (pool.head_dim) {
-    case 64: return run_fp8<T, 64>(pool, a, stream);
-    case 128: return run_fp8<T, 128>(pool, a, stream);
-    default: return run_fp8<T, 256>(pool, a, stream);
+    case 64: return run_fp8_scores<T, 64>(pool, a, stream);
+    case 128: return run_fp8_scores<T, 128>(pool, a, stream);
+    default: return run_fp8_scores<T, 256>(pool, a, stream);
   }
 }
 
 int launch_fp8_decode(const clove_fp8_pool& pool, const Fp8DecodeCall& c, cudaStream_t stream) {
   const Fp8Layout L = fp8_layout(pool, c.batch, c.num_q_heads, c.max_ctx, c.scores.accumulate);
   unsigned char* ws = static_cast<unsigned char*>(c.workspace);
-  const int slice = std::min(pool.block_size, kSlice);
+  const int slice = std::min(pool.block_size, stage_tokens(pool.head_dim));
   Fp8Args a = {};
   a.q = c.q;
   a.k_new = c.k_new;
@@ -1021,7 +1333,8 @@ int launch_fp8_decode(const clove_fp8_pool& pool, const Fp8DecodeCall& c, cudaSt
   a.mass = pool.mass;
   a.slopes = c.scores.alibi_slopes;
   a.real_block = pool.block_size;
-  for (a.sub_shift = 0; (slice << a.sub_shift) < pool.block_size;) ++a.sub_shift;
+  while ((1 << a.slice_shift) < slice) ++a.slice_shift;
+  while ((1 << a.real_shift) < pool.block_size) ++a.real_shift;
   a.window = c.scores.window;
   a.scale = c.scale;
   a.softcap = c.scores.softcap;
@@ -1031,7 +1344,7 @@ int launch_fp8_decode(const clove_fp8_pool& pool, const Fp8DecodeCall& c, cudaSt
     a.z_stride = L.z_stride;
   }
   a.direct = 0;
-  a.append_here = a.append && (a.direct || a.sub_shift == 0);
+  a.append_here = a.append && (a.direct || slice == pool.block_size);
   switch (c.dtype) {
     case CLOVE_DTYPE_F32: return run_fp8_dim<float>(pool, a, stream);
     case CLOVE_DTYPE_F16: return run_fp8_dim<__half>(pool, a, stream);

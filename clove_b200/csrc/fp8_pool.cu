@@ -76,7 +76,7 @@ int finish_pool(clove_fp8_pool* p) {
   if (e != cudaSuccess) return cuda_fail("cudaMalloc(flags)", e);
   e = cudaMemset(p->flags, 0, 256);
   if (e != cudaSuccess) return cuda_fail("cudaMemset(flags)", e);
-  return fp8_encode_maps(*p);
+  return fp8_encode_map(*p);
 }
 
 // Tables, lengths and bounds that every reading call takes.
