@@ -20,6 +20,7 @@ struct clove_fp8_pool {
   float* mass;           // [num_blocks, num_kv_heads, block_size] or null
   size_t plane_bytes;    // bytes of one plane of codes
   int32_t* flags;        // device word: check flags of all calls
+  int32_t* slot_token;   // append index: a word per slot, then one per block; zero between calls
   int num_sms;
   CUtensorMap map;  // the codes as the decode's copies see them
 };
@@ -86,6 +87,9 @@ struct Fp8AppendArgs {
   float* scales;
   float* mass;
   int32_t* flags;
+  int32_t* slot_token;   // the pool's append index
+  int32_t* block_state;
+  int32_t* leads;        // [tokens] workspace
   size_t plane_bytes;
   int num_tokens, num_blocks, block_size, num_kv_heads;
 };

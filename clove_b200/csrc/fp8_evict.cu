@@ -1,10 +1,16 @@
 // Eviction by accumulated attention weight.
 //
-// select    one CTA per (sequence, KV head): radix selection of the weight of
-//           the last token kept (8 bits of the key per pass), then an ordered
-//           write of the kept indices.
-// compact   one CTA per (new block, KV head, sequence): gathers the kept rows
+// select    a cluster of 1 to 8 CTAs per (sequence, KV head), each with a part
+//           of the tokens.  The weights become ordered 32-bit keys, read from
+//           HBM once and kept in shared memory; three histograms of 11, 11 and
+//           10 bits, summed over the cluster through distributed shared memory,
+//           find the key of the last token kept; then every warp writes its
+//           kept tokens at their place, counted from the parts before it.
+// compact   one warp per (new block, KV head, sequence): gathers the kept rows
 //           into the new block, rounding to its scale where that is larger.
+//           All loads of 16 rows are under way at once.
+// HBM bounds both: 4 bytes per token and KV head for the first, 4 head_dim
+// bytes per kept token and KV head (read and written, K and V) for the second.
 #include <algorithm>
 
 #include "fp8_common.cuh"
@@ -36,9 +42,12 @@ __device__ __forceinline__ int evict_len(const Fp8EvictArgs& a, int b) {
   return max(0, min(__ldg(a.context_lens + b), a.max_ctx));
 }
 
-constexpr int kSelThreads = 1024;
+constexpr int kSelThreads = 512, kSelWarps = kSelThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kMaxRoom = 48 * 1024;
 
-__device__ __forceinline__ int block_scan(int x, int* warp_tot, int* total) {  // exclusive
+// Exclusive sum over the block of one int per thread; *total gets the sum.
+__device__ __forceinline__ int block_scan(int x, int* warp_tot, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int s = x;
 #pragma unroll
@@ -46,140 +55,253 @@ __device__ __forceinline__ int block_scan(int x, int* warp_tot, int* total) {  /
     const int y = __shfl_up_sync(0xffffffffu, s, o);
     if (lane >= o) s += y;
   }
-  __syncthreads();
   if (lane == 31) warp_tot[warp] = s;
   __syncthreads();
-  if (warp == 0) {
-    int w = lane < kSelThreads / 32 ? warp_tot[lane] : 0;
+  int before = 0, all = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += y;
-    }
-    warp_tot[lane] = w;
+  for (int w = 0; w < kSelWarps; ++w) {
+    if (w < warp) before += warp_tot[w];
+    all += warp_tot[w];
   }
+  *total = all;
   __syncthreads();
-  *total = warp_tot[kSelThreads / 32 - 1];
-  return s - x + (warp > 0 ? warp_tot[warp - 1] : 0);
+  return before + s - x;
 }
 
-__global__ void __launch_bounds__(kSelThreads) fp8_select_kernel(const Fp8EvictArgs a) {
-  __shared__ int hist[256];
-  __shared__ int warp_tot[32];
-  __shared__ int s_digit, s_above;
-  const int h = blockIdx.x, b = blockIdx.y, H = a.num_kv_heads, bs = a.block_size, tid = threadIdx.x;
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// The address of `p` (shared) in CTA `rank` of the cluster, and a read of it.
+__device__ __forceinline__ uint32_t peer_address(const void* p, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ int4 peer_int4(uint32_t a) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ int2 peer_int2(uint32_t a) {
+  int2 v;
+  asm volatile("ld.shared::cluster.v2.s32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+
+// Grid (C * heads, batch), clusters of C along x.  `room`: keys that the
+// dynamic shared memory holds; a part longer than that is read from the cache
+// again in every pass.
+__global__ void __launch_bounds__(kSelThreads) fp8_select_kernel(const Fp8EvictArgs a, int C, int room) {
+  extern __shared__ uint32_t keys[];
+  __shared__ __align__(16) int hist[kBins];
+  __shared__ int warp_tot[kSelWarps];
+  __shared__ int2 warp_cnt[kSelWarps];       // keys above and equal to the threshold
+  __shared__ __align__(8) int2 part_cnt;     // the same of this CTA
+  __shared__ __align__(8) int2 found;        // digit, keys above it
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int h = blockIdx.x / C, rank = blockIdx.x - h * C, b = blockIdx.y, H = a.num_kv_heads, bs = a.block_size;
+  const int shift = 31 - __clz(bs);
+  griddep_wait();
   const int n = evict_len(a, b), m = min(n, a.budget);
-  if (h == 0 && tid == 0) {
+  if (h == 0 && rank == 0 && tid == 0) {
     a.new_lens[b] = m;
     if (__ldg(a.context_lens + b) != n) atomicOr(a.flags, CLOVE_FLAG_CTX_RANGE);
   }
   int32_t* kept = a.kept + ((size_t)b * H + h) * a.budget;
-  for (int i = m + tid; i < a.budget; i += kSelThreads) kept[i] = -1;
+  const int self = rank * kSelThreads + tid, all = C * kSelThreads;
+  for (int i = m + self; i < a.budget; i += all) kept[i] = -1;
   const int last = min(a.recent, n), old = n - last, need = m - last;
-  for (int i = tid; i < last; i += kSelThreads) kept[need + i] = old + i;
-  if (need == 0) return;
+  for (int i = self; i < last; i += all) kept[need + i] = old + i;
+  if (need == 0) return;  // (every CTA of the cluster alike)
   if (need == old) {
-    for (int i = tid; i < need; i += kSelThreads) kept[i] = i;
+    for (int i = self; i < need; i += all) kept[i] = i;
     return;
   }
   const int32_t* table = a.block_tables + (size_t)b * a.bt_stride;
-  auto key = [&](int t) {
-    int blk = __ldg(table + t / bs);
+  auto load = [&](int t) {
+    int blk = __ldg(table + (t >> shift));
     if (blk < 0 || blk >= a.num_blocks) {
       atomicOr(a.flags, CLOVE_FLAG_BLOCK_OOB);
       blk = 0;
     }
-    return mass_key(a.mass[((size_t)blk * H + h) * bs + t % bs]);
+    return mass_key(__ldg(a.mass + ((size_t)blk * H + h) * bs + (t & (bs - 1))));
   };
-  // the need-th largest key, 8 bits at a time
+  // this CTA's tokens [t0, t1), a multiple of 32 per warp
+  const int part = ((old + C - 1) / C + kSelThreads - 1) / kSelThreads * kSelThreads;
+  const int t0 = min(old, rank * part), t1 = min(old, t0 + part), cnt = t1 - t0;
+  const bool held = cnt <= room;
+  if (held) {
+#pragma unroll 4
+    for (int i = tid; i < cnt; i += kSelThreads) keys[i] = load(t0 + i);
+  }
+  auto key = [&](int i) { return held ? keys[i] : load(t0 + i); };
+
+  // ---- the need-th largest key ----
   uint32_t prefix = 0;
   int left = need;  // rank of the wanted key among those that share the prefix
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int low = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
     __syncthreads();
-    for (int t = tid; t < old; t += kSelThreads) {
-      const uint32_t k = key(t);
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+    for (int i = tid; i < cnt; i += kSelThreads) {
+      const uint32_t k = key(i);
+      if (pass == 0 || ((k ^ prefix) >> (low + bits)) == 0) atomicAdd(&hist[(k >> low) & ((1u << bits) - 1)], 1);
     }
-    __syncthreads();
-    int total;
-    const int c = tid < 256 ? hist[255 - tid] : 0;  // from the largest digit down
-    const int above = block_scan(c, warp_tot, &total);
-    if (tid < 256 && above < left && left <= above + c) {
-      s_digit = 255 - tid;
-      s_above = above;
+    if (C > 1) cluster_sync();
+    else __syncthreads();
+    if (rank == 0) {
+      // thread i: four bins, from the largest down
+      const int first = kBins - 4 - 4 * tid;
+      int4 c = *reinterpret_cast<const int4*>(hist + first);
+      for (int r = 1; r < C; ++r) {
+        const int4 p = peer_int4(peer_address(hist + first, r));
+        c.x += p.x;
+        c.y += p.y;
+        c.z += p.z;
+        c.w += p.w;
+      }
+      int total;
+      int above = block_scan(c.x + c.y + c.z + c.w, warp_tot, &total);
+      const int v[4] = {c.w, c.z, c.y, c.x};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (above < left && left <= above + v[k]) found = make_int2(first + 3 - k, above);
+        above += v[k];
+      }
     }
-    __syncthreads();
-    prefix |= (uint32_t)s_digit << shift;
-    left -= s_above;
-    __syncthreads();
+    if (C > 1) cluster_sync();
+    else __syncthreads();
+    const int2 f = C > 1 ? peer_int2(peer_address(&found, 0)) : found;
+    prefix |= (uint32_t)f.x << low;
+    left -= f.y;
+    if (C > 1) cluster_sync();  // (rank 0 may not change `found` before all have read it)
+    else __syncthreads();
   }
-  // keys above the threshold, and the first `left` of those equal to it
-  int at = 0, equal = 0;
-  for (int base = 0; base < old; base += kSelThreads) {
-    const int t = base + tid;
-    const uint32_t k = t < old ? key(t) : 0u;
-    const int eq = t < old && k == prefix;
-    int neq, nkeep;
-    const int r = equal + block_scan(eq, warp_tot, &neq);
-    const int keep = t < old && (k > prefix || (eq && r < left));
-    const int pos = at + block_scan(keep, warp_tot, &nkeep);
-    if (keep) kept[pos] = t;
-    equal += neq;
-    at += nkeep;
+
+  // ---- the keys above the threshold, and the first `left` of those equal to it ----
+  const int per_warp = part / kSelWarps, w0 = warp * per_warp, w1 = min(cnt, w0 + per_warp);
+  int gt = 0, eq = 0;
+  for (int base = w0; base < w1; base += 32) {
+    const bool in = base + lane < w1;
+    const uint32_t k = in ? key(base + lane) : 0u;
+    gt += __popc(__ballot_sync(0xffffffffu, in && k > prefix));
+    eq += __popc(__ballot_sync(0xffffffffu, in && k == prefix));
+  }
+  if (lane == 0) warp_cnt[warp] = make_int2(gt, eq);
+  __syncthreads();
+  int2 sum = make_int2(0, 0), before = make_int2(0, 0);
+  for (int w = 0; w < kSelWarps; ++w) {
+    if (w == warp) before = sum;
+    sum.x += warp_cnt[w].x;
+    sum.y += warp_cnt[w].y;
+  }
+  if (C > 1) {
+    if (tid == 0) part_cnt = sum;
+    cluster_sync();
+    for (int r = 0; r < rank; ++r) {
+      const int2 p = peer_int2(peer_address(&part_cnt, r));
+      before.x += p.x;
+      before.y += p.y;
+    }
+    cluster_sync();  // no CTA leaves while its shared memory is read
+  }
+  const unsigned lower = (1u << lane) - 1;
+  for (int base = w0; base < w1; base += 32) {
+    const bool in = base + lane < w1;
+    const uint32_t k = in ? key(base + lane) : 0u;
+    const unsigned mg = __ballot_sync(0xffffffffu, in && k > prefix), me = __ballot_sync(0xffffffffu, in && k == prefix);
+    const int g = before.x + __popc(mg & lower), e = before.y + __popc(me & lower);
+    if (in && (k > prefix || (k == prefix && e < left))) kept[g + min(e, left)] = t0 + base + lane;
+    before.x += __popc(mg);
+    before.y += __popc(me);
   }
 }
 
-constexpr int kCompactThreads = 128;
+constexpr int kCompactWarps = 4;
+
+// Two 16-byte pieces of codes to a scale 1 / ratio times as large.
+__device__ __forceinline__ uint4 fp8_rescale16(uint4 c, float ratio) {
+  const uint2 lo = fp8_rescale8(make_uint2(c.x, c.y), ratio), hi = fp8_rescale8(make_uint2(c.z, c.w), ratio);
+  return make_uint4(lo.x, lo.y, hi.x, hi.y);
+}
 
 template <int D>
-__global__ void __launch_bounds__(kCompactThreads) fp8_compact_kernel(const Fp8EvictArgs a) {
-  constexpr int LPR = D / 8;
-  __shared__ int row[256];      // source row (tile * block_size + offset) of each new row, -1: bad block
-  __shared__ float sc[2][256];  // its scales
-  __shared__ float top[2];
-  const int j = blockIdx.x, h = blockIdx.y, b = blockIdx.z, H = a.num_kv_heads, bs = a.block_size;
-  const int tid = threadIdx.x;
+__global__ void __launch_bounds__(kCompactWarps * 32) fp8_compact_kernel(const Fp8EvictArgs a) {
+  constexpr int LPR = D / 16, RPW = 32 / LPR, STEP = 16 / RPW;  // lanes per row, rows per load, loads of 16 rows
+  const int lane = threadIdx.x & 31, sub = lane % LPR, r0 = lane / LPR;
+  const int j = blockIdx.x * kCompactWarps + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
+  const int H = a.num_kv_heads, bs = a.block_size, shift = 31 - __clz(bs);
+  griddep_wait();
   const int m = min(evict_len(a, b), a.budget), first = j * bs, rows = min(bs, m - first);
   if (rows <= 0) return;
   const int dst = __ldg(a.new_tables + (size_t)b * a.new_stride + j);
   if (dst < 0 || dst >= a.num_blocks) {
-    if (tid == 0 && h == 0) atomicOr(a.flags, CLOVE_FLAG_BLOCK_OOB);
+    if (lane == 0 && h == 0) atomicOr(a.flags, CLOVE_FLAG_BLOCK_OOB);
     return;
   }
-  const size_t to = (size_t)dst * H + h;
+  const size_t to = (size_t)dst * H + h, plane = (size_t)a.num_blocks * H;
   const int32_t* kept = a.kept + ((size_t)b * H + h) * a.budget + first;
-  for (int r = tid; r < rows; r += kCompactThreads) {
-    const int t = kept[r];
-    int blk = __ldg(a.block_tables + (size_t)b * a.bt_stride + t / bs);
-    if (blk < 0 || blk >= a.num_blocks) {
-      atomicOr(a.flags, CLOVE_FLAG_BLOCK_OOB);
-      blk = 0;
+  // lane r: source tile and offset of row base + r, and its scales
+  struct Source {
+    int row;
+    float s[2];
+  };
+  auto source = [&](int r, bool move_mass) {
+    Source s = {0, {0.f, 0.f}};
+    if (r < rows) {
+      const int t = __ldcg(kept + r);
+      int blk = __ldg(a.block_tables + (size_t)b * a.bt_stride + (t >> shift));
+      if (blk < 0 || blk >= a.num_blocks) {
+        atomicOr(a.flags, CLOVE_FLAG_BLOCK_OOB);
+        blk = 0;
+      }
+      const size_t tile = (size_t)blk * H + h;
+      s.row = (int)(tile * bs) + (t & (bs - 1));
+      s.s[0] = a.scales[tile];
+      s.s[1] = a.scales[plane + tile];
+      if (move_mass) a.mass[to * bs + r] = a.mass[s.row];
     }
-    const size_t tile = (size_t)blk * H + h;
-    row[r] = (int)(tile * bs) + t % bs;
-    sc[0][r] = a.scales[tile];
-    sc[1][r] = a.scales[(size_t)a.num_blocks * H + tile];
-    a.mass[to * bs + r] = a.mass[tile * bs + t % bs];
+    return s;
+  };
+  Source now = source(lane, true);
+  float top[2] = {now.s[0], now.s[1]};
+  for (int base = 32; base < rows; base += 32) {
+    const Source s = source(base + lane, true);
+    top[0] = fmaxf(top[0], s.s[0]);
+    top[1] = fmaxf(top[1], s.s[1]);
   }
-  __syncthreads();
-  if (tid < 64) {
-    float x = 0.f;
-    for (int r = tid & 31; r < rows; r += 32) x = fmaxf(x, sc[tid >> 5][r]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-    if ((tid & 31) == 0) {
-      top[tid >> 5] = x;
-      a.scales[(size_t)(tid >> 5) * a.num_blocks * H + to] = x;
-    }
+  for (int p = 0; p < 2; ++p) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top[p] = fmaxf(top[p], __shfl_xor_sync(0xffffffffu, top[p], o));
+    if (lane == 0) a.scales[p * plane + to] = top[p];
   }
-  __syncthreads();
-  for (int i = tid; i < 2 * rows * LPR; i += kCompactThreads) {
-    const int p = i / (rows * LPR), k = i - p * rows * LPR, r = k / LPR, w = k - r * LPR;
-    unsigned char* plane = a.codes + p * a.plane_bytes;
-    uint2 x = *reinterpret_cast<const uint2*>(plane + (size_t)row[r] * D + w * 8);
-    if (sc[p][r] != top[p]) x = fp8_rescale8(x, sc[p][r] / top[p]);
-    *reinterpret_cast<uint2*>(plane + (to * bs + r) * D + w * 8) = x;
+  for (int base = 0; base < rows; base += 32) {
+    if (base > 0) now = source(base + lane, false);
+    for (int half = 0; half < 32 && base + half < rows; half += 16) {
+      uint4 c[2][STEP];
+#pragma unroll
+      for (int i = 0; i < STEP; ++i) {
+        const int r = half + i * RPW + r0, src = __shfl_sync(0xffffffffu, now.row, r);
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          if (base + r < rows)
+            c[p][i] = *reinterpret_cast<const uint4*>(a.codes + p * a.plane_bytes + (size_t)src * D + sub * 16);
+      }
+#pragma unroll
+      for (int i = 0; i < STEP; ++i) {
+        const int r = half + i * RPW + r0;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const float s = __shfl_sync(0xffffffffu, now.s[p], r);
+          if (base + r < rows) {
+            if (s != top[p]) c[p][i] = fp8_rescale16(c[p][i], s / top[p]);
+            *reinterpret_cast<uint4*>(a.codes + p * a.plane_bytes + (to * bs + base + r) * D + sub * 16) = c[p][i];
+          }
+        }
+      }
+    }
   }
 }
 
@@ -205,20 +327,46 @@ int launch_fp8_evict(const clove_fp8_pool& pool, const Fp8EvictCall& c, cudaStre
   a.num_blocks = pool.num_blocks;
   a.block_size = pool.block_size;
   a.num_kv_heads = pool.num_kv_heads;
-  fp8_select_kernel<<<dim3(pool.num_kv_heads, c.batch), kSelThreads, 0, stream>>>(a);
-  int rc = fp8_launch_status("fp8_evict select launch", cudaGetLastError());
+  // CTAs per (sequence, head): parts of at most 8192 tokens of the longest sequence, in a cluster of up to 8.  Keys
+  // that fit stay in shared memory (room for 8192 to 48 K of them); longer parts are read again.
+  const int most = std::min(c.budget, c.max_ctx);
+  int C = 1;
+  while (C < 8 && (long long)C * 8192 < c.max_ctx) C *= 2;
+  const int part = ((c.max_ctx + C - 1) / C + kSelThreads - 1) / kSelThreads * kSelThreads;
+  const int room = part <= kMaxRoom ? part : 0, smem = room * (int)sizeof(uint32_t);
+  int rc = fp8_launch_status("cudaFuncSetAttribute", cudaFuncSetAttribute(fp8_select_kernel,
+                                                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                                          kMaxRoom * (int)sizeof(uint32_t)));
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(C * pool.num_kv_heads, c.batch);
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {(unsigned)C, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  rc = fp8_launch_status("fp8_evict select launch", cudaLaunchKernelEx(&cfg, fp8_select_kernel, a, C, room));
   if (rc) return rc;
   count_launches(1);
-  const int most = std::min(c.budget, c.max_ctx);
   if (most == 0) return CLOVE_OK;
-  const dim3 grid((most + pool.block_size - 1) / pool.block_size, pool.num_kv_heads, c.batch);
+  const int blocks = (most + pool.block_size - 1) / pool.block_size;
+  cfg.gridDim = dim3((blocks + kCompactWarps - 1) / kCompactWarps, pool.num_kv_heads, c.batch);
+  cfg.blockDim = dim3(kCompactWarps * 32);
+  cfg.dynamicSmemBytes = 0;
+  cfg.numAttrs = 1;
+  cudaError_t e;
   switch (pool.head_dim) {
-    case 64: fp8_compact_kernel<64><<<grid, kCompactThreads, 0, stream>>>(a); break;
-    case 128: fp8_compact_kernel<128><<<grid, kCompactThreads, 0, stream>>>(a); break;
-    default: fp8_compact_kernel<256><<<grid, kCompactThreads, 0, stream>>>(a); break;
+    case 64: e = cudaLaunchKernelEx(&cfg, fp8_compact_kernel<64>, a); break;
+    case 128: e = cudaLaunchKernelEx(&cfg, fp8_compact_kernel<128>, a); break;
+    default: e = cudaLaunchKernelEx(&cfg, fp8_compact_kernel<256>, a); break;
   }
   count_launches(1);
-  return fp8_launch_status("fp8_evict compact launch", cudaGetLastError());
+  return fp8_launch_status("fp8_evict compact launch", e);
 }
 
 }  // namespace clove

@@ -76,6 +76,15 @@ int finish_pool(clove_fp8_pool* p) {
   if (e != cudaSuccess) return cuda_fail("cudaMalloc(flags)", e);
   e = cudaMemset(p->flags, 0, 256);
   if (e != cudaSuccess) return cuda_fail("cudaMemset(flags)", e);
+  const size_t index = sizeof(int32_t) * (size_t)p->num_blocks * (p->block_size + 1);
+  e = cudaMalloc(reinterpret_cast<void**>(&p->slot_token), index);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_last_error("cudaMalloc(append index, %zu): %s", index, cudaGetErrorString(e));
+    return CLOVE_ERR_OOM;
+  }
+  e = cudaMemset(p->slot_token, 0, index);
+  if (e != cudaSuccess) return cuda_fail("cudaMemset(append index)", e);
   return fp8_encode_map(*p);
 }
 
@@ -179,6 +188,7 @@ int clove_fp8_pool_destroy(clove_fp8_pool_t pool) {
   OnDevice g(pool->device);
   if (pool->owns_memory) cudaFree(pool->codes);
   if (pool->flags) cudaFree(pool->flags);
+  if (pool->slot_token) cudaFree(pool->slot_token);
   delete pool;
   return CLOVE_OK;
 }

@@ -77,7 +77,7 @@ typedef struct clove_fp8_scores {
 /* Allocate a cache (codes, scales and, with with_mass, mass; all zero), or
  * wrap caller-owned device arrays (codes 128-byte aligned, scales and mass
  * 16-byte aligned; mass may be null) without taking ownership.  Both allocate
- * the pool's status word. */
+ * the pool's status word and its append index (4 bytes per token slot). */
 int clove_fp8_pool_create(int device, int num_blocks, int block_size, int num_kv_heads, int head_dim,
                           int with_mass, clove_fp8_pool_t* out);
 int clove_fp8_pool_wrap(int device, void* codes, float* scales, float* mass, int num_blocks, int block_size,
