@@ -6,9 +6,11 @@
 //           10 bits, summed over the cluster through distributed shared memory,
 //           find the key of the last token kept; then every warp writes its
 //           kept tokens at their place, counted from the parts before it.
-// compact   one warp per (new block, KV head, sequence): gathers the kept rows
-//           into the new block, rounding to its scale where that is larger.
-//           All loads of 16 rows are under way at once.
+// compact   a warp moves 32 kept rows of a (sequence, KV head) at a time into
+//           their new blocks, rounding to a new block's scale where that is
+//           larger; the loads of 32 rows (16 at head_dim 256) are under way at
+//           once, and beside them the chain (kept index, table, scales) that
+//           the warp's next rows need.
 // HBM bounds both: 4 bytes per token and KV head for the first, 4 head_dim
 // bytes per kept token and KV head (read and written, K and V) for the second.
 #include <algorithm>
@@ -42,11 +44,11 @@ __device__ __forceinline__ int evict_len(const Fp8EvictArgs& a, int b) {
   return max(0, min(__ldg(a.context_lens + b), a.max_ctx));
 }
 
-constexpr int kSelThreads = 512, kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kMaxRoom = 48 * 1024;
+constexpr int kMaxRoom = 16 * 1024;  // keys in shared memory: three CTAs on an SM
 
 // Exclusive sum over the block of one int per thread; *total gets the sum.
+template <int kSelWarps>
 __device__ __forceinline__ int block_scan(int x, int* warp_tot, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int s = x;
@@ -89,15 +91,17 @@ __device__ __forceinline__ int2 peer_int2(uint32_t a) {
 }
 
 // Grid (C * heads, batch), clusters of C along x.  `room`: keys that the
-// dynamic shared memory holds; a part longer than that is read from the cache
-// again in every pass.
-__global__ void __launch_bounds__(kSelThreads) fp8_select_kernel(const Fp8EvictArgs a, int C, int room) {
+// dynamic shared memory holds; what a part has beyond that is read from the
+// cache (L2) again in every pass.
+template <int kSelThreads, int kPerSm>
+__global__ void __launch_bounds__(kSelThreads, kPerSm) fp8_select_kernel(const Fp8EvictArgs a, int C, int room) {
+  constexpr int kSelWarps = kSelThreads / 32, kBinsPer = kBins / kSelThreads;
   extern __shared__ uint32_t keys[];
   __shared__ __align__(16) int hist[kBins];
   __shared__ int warp_tot[kSelWarps];
   __shared__ int2 warp_cnt[kSelWarps];       // keys above and equal to the threshold
   __shared__ __align__(8) int2 part_cnt;     // the same of this CTA
-  __shared__ __align__(8) int2 found;        // digit, keys above it
+  __shared__ __align__(16) int4 found;       // digit, keys above it, keys with it
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int h = blockIdx.x / C, rank = blockIdx.x - h * C, b = blockIdx.y, H = a.num_kv_heads, bs = a.block_size;
   const int shift = 31 - __clz(bs);
@@ -129,12 +133,9 @@ __global__ void __launch_bounds__(kSelThreads) fp8_select_kernel(const Fp8EvictA
   // this CTA's tokens [t0, t1), a multiple of 32 per warp
   const int part = ((old + C - 1) / C + kSelThreads - 1) / kSelThreads * kSelThreads;
   const int t0 = min(old, rank * part), t1 = min(old, t0 + part), cnt = t1 - t0;
-  const bool held = cnt <= room;
-  if (held) {
 #pragma unroll 4
-    for (int i = tid; i < cnt; i += kSelThreads) keys[i] = load(t0 + i);
-  }
-  auto key = [&](int i) { return held ? keys[i] : load(t0 + i); };
+  for (int i = tid; i < min(cnt, room); i += kSelThreads) keys[i] = load(t0 + i);
+  auto key = [&](int i) { return i < room ? keys[i] : load(t0 + i); };
 
   // ---- the need-th largest key ----
   uint32_t prefix = 0;
@@ -151,30 +152,43 @@ __global__ void __launch_bounds__(kSelThreads) fp8_select_kernel(const Fp8EvictA
     if (C > 1) cluster_sync();
     else __syncthreads();
     if (rank == 0) {
-      // thread i: four bins, from the largest down
-      const int first = kBins - 4 - 4 * tid;
-      int4 c = *reinterpret_cast<const int4*>(hist + first);
-      for (int r = 1; r < C; ++r) {
-        const int4 p = peer_int4(peer_address(hist + first, r));
-        c.x += p.x;
-        c.y += p.y;
-        c.z += p.z;
-        c.w += p.w;
+      // thread i: kBinsPer bins, from the largest down
+      const int first = kBins - kBinsPer * (tid + 1);
+      int v[kBinsPer], mine = 0;
+#pragma unroll
+      for (int k = 0; k < kBinsPer; k += 4) {
+        int4 c = *reinterpret_cast<const int4*>(hist + first + k);
+        for (int r = 1; r < C; ++r) {
+          const int4 p = peer_int4(peer_address(hist + first + k, r));
+          c.x += p.x;
+          c.y += p.y;
+          c.z += p.z;
+          c.w += p.w;
+        }
+        v[k] = c.x;
+        v[k + 1] = c.y;
+        v[k + 2] = c.z;
+        v[k + 3] = c.w;
+        mine += c.x + c.y + c.z + c.w;
       }
       int total;
-      int above = block_scan(c.x + c.y + c.z + c.w, warp_tot, &total);
-      const int v[4] = {c.w, c.z, c.y, c.x};
+      int above = block_scan<kSelWarps>(mine, warp_tot, &total);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (above < left && left <= above + v[k]) found = make_int2(first + 3 - k, above);
+      for (int k = kBinsPer - 1; k >= 0; --k) {
+        if (above < left && left <= above + v[k]) found = make_int4(first + k, above, v[k], 0);
         above += v[k];
       }
     }
     if (C > 1) cluster_sync();
     else __syncthreads();
-    const int2 f = C > 1 ? peer_int2(peer_address(&found, 0)) : found;
+    const int4 f = C > 1 ? peer_int4(peer_address(&found, 0)) : found;
     prefix |= (uint32_t)f.x << low;
     left -= f.y;
+    if (left == f.z && prefix > 0) {  // all keys with these digits are kept
+      --prefix;
+      left = 0;
+      break;
+    }
     if (C > 1) cluster_sync();  // (rank 0 may not change `found` before all have read it)
     else __syncthreads();
   }
@@ -218,7 +232,7 @@ __global__ void __launch_bounds__(kSelThreads) fp8_select_kernel(const Fp8EvictA
   }
 }
 
-constexpr int kCompactWarps = 4;
+constexpr int kCompactWarps = 4, kCompactPerSm = 5;
 
 // Two 16-byte pieces of codes to a scale 1 / ratio times as large.
 __device__ __forceinline__ uint4 fp8_rescale16(uint4 c, float ratio) {
@@ -226,82 +240,119 @@ __device__ __forceinline__ uint4 fp8_rescale16(uint4 c, float ratio) {
   return make_uint4(lo.x, lo.y, hi.x, hi.y);
 }
 
+// A warp's item: 32 kept rows of one (sequence, KV head).  `chunks`: items of a
+// (sequence, head), enough for the longest one.
 template <int D>
-__global__ void __launch_bounds__(kCompactWarps * 32) fp8_compact_kernel(const Fp8EvictArgs a) {
-  constexpr int LPR = D / 16, RPW = 32 / LPR, STEP = 16 / RPW;  // lanes per row, rows per load, loads of 16 rows
+__global__ void __launch_bounds__(kCompactWarps * 32, kCompactPerSm)
+    fp8_compact_kernel(const Fp8EvictArgs a, int batch, int chunks) {
+  constexpr int LPR = D / 16, RPW = 32 / LPR;         // lanes per row, rows per load
+  constexpr int STEP = D == 64 ? 4 : 8, ROWS = STEP * RPW;  // loads per plane and rows per batch
   const int lane = threadIdx.x & 31, sub = lane % LPR, r0 = lane / LPR;
-  const int j = blockIdx.x * kCompactWarps + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
   const int H = a.num_kv_heads, bs = a.block_size, shift = 31 - __clz(bs);
+  const size_t plane = (size_t)a.num_blocks * H;
   griddep_wait();
-  const int m = min(evict_len(a, b), a.budget), first = j * bs, rows = min(bs, m - first);
-  if (rows <= 0) return;
-  const int dst = __ldg(a.new_tables + (size_t)b * a.new_stride + j);
-  if (dst < 0 || dst >= a.num_blocks) {
-    if (lane == 0 && h == 0) atomicOr(a.flags, CLOVE_FLAG_BLOCK_OOB);
-    return;
-  }
-  const size_t to = (size_t)dst * H + h, plane = (size_t)a.num_blocks * H;
-  const int32_t* kept = a.kept + ((size_t)b * H + h) * a.budget + first;
-  // lane r: source tile and offset of row base + r, and its scales
-  struct Source {
-    int row;
-    float s[2];
+  const int total = batch * H * chunks, stride = gridDim.x * kCompactWarps;
+
+  // Lane r of an item: row `from` (tile * block_size + offset) goes to row
+  // `to`, its codes times ratio (K, V) rounded; to < 0: nothing.
+  struct Move {
+    int from, to;
+    float ratio[2];
   };
-  auto source = [&](int r, bool move_mass) {
-    Source s = {0, {0.f, 0.f}};
-    if (r < rows) {
-      const int t = __ldcg(kept + r);
-      int blk = __ldg(a.block_tables + (size_t)b * a.bt_stride + (t >> shift));
-      if (blk < 0 || blk >= a.num_blocks) {
-        atomicOr(a.flags, CLOVE_FLAG_BLOCK_OOB);
-        blk = 0;
-      }
-      const size_t tile = (size_t)blk * H + h;
-      s.row = (int)(tile * bs) + (t & (bs - 1));
-      s.s[0] = a.scales[tile];
-      s.s[1] = a.scales[plane + tile];
-      if (move_mass) a.mass[to * bs + r] = a.mass[s.row];
+  auto scales_of = [&](int b, int h, int t, float (&s)[2]) {
+    int blk = __ldg(a.block_tables + (size_t)b * a.bt_stride + (t >> shift));
+    if (blk < 0 || blk >= a.num_blocks) {
+      atomicOr(a.flags, CLOVE_FLAG_BLOCK_OOB);
+      blk = 0;
     }
-    return s;
+    const int tile = blk * H + h;
+    s[0] = a.scales[tile];
+    s[1] = a.scales[plane + tile];
+    return tile * bs + (t & (bs - 1));
   };
-  Source now = source(lane, true);
-  float top[2] = {now.s[0], now.s[1]};
-  for (int base = 32; base < rows; base += 32) {
-    const Source s = source(base + lane, true);
-    top[0] = fmaxf(top[0], s.s[0]);
-    top[1] = fmaxf(top[1], s.s[1]);
-  }
-#pragma unroll
-  for (int p = 0; p < 2; ++p) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top[p] = fmaxf(top[p], __shfl_xor_sync(0xffffffffu, top[p], o));
-    if (lane == 0) a.scales[p * plane + to] = top[p];
-  }
-  for (int base = 0; base < rows; base += 32) {
-    if (base > 0) now = source(base + lane, false);
-    for (int half = 0; half < 32 && base + half < rows; half += 16) {
-      uint4 c[2][STEP];
-#pragma unroll
-      for (int i = 0; i < STEP; ++i) {
-        const int r = half + i * RPW + r0, src = __shfl_sync(0xffffffffu, now.row, r);
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-          if (base + r < rows)
-            c[p][i] = *reinterpret_cast<const uint4*>(a.codes + p * a.plane_bytes + (size_t)src * D + sub * 16);
+  auto prepare = [&](int item) {
+    Move v = {0, -1, {1.f, 1.f}};
+    if (item >= total) return v;
+    const int head = item / chunks, r = (item - head * chunks) * 32 + lane, b = head / H, h = head - b * H;
+    const int m = min(evict_len(a, b), a.budget);
+    if ((r & ~31) >= m) return v;
+    const int32_t* kept = a.kept + (size_t)head * a.budget;
+    float s[2] = {0.f, 0.f}, top[2];
+    int dst = -1;
+    if (r < m) {
+      dst = __ldg(a.new_tables + (size_t)b * a.new_stride + (r >> shift));
+      v.from = scales_of(b, h, __ldcg(kept + r), s);
+    }
+    // the new block's scale: the largest of its rows'
+    top[0] = s[0];
+    top[1] = s[1];
+    if (bs > 32) {
+      const int first = r >> shift << shift;
+      for (int k = first - (first & 31) + lane; k < min(m, first + bs); k += 32) {
+        float o[2];
+        scales_of(b, h, __ldcg(kept + k), o);
+        top[0] = fmaxf(top[0], o[0]);
+        top[1] = fmaxf(top[1], o[1]);
       }
+    }
+    for (int o = min(bs, 32) / 2; o > 0; o >>= 1) {
+      top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
+      top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
+    }
+    if (r < m) {
+      if (dst < 0 || dst >= a.num_blocks) {
+        atomicOr(a.flags, CLOVE_FLAG_BLOCK_OOB);
+      } else {
+        const int tile = dst * H + h, off = r & (bs - 1);
+        v.to = tile * bs + off;
+        if (off == 0) {
+          a.scales[tile] = top[0];
+          a.scales[plane + tile] = top[1];
+        }
+        a.mass[v.to] = a.mass[v.from];
+        if (s[0] != top[0]) v.ratio[0] = s[0] / top[0];
+        if (s[1] != top[1]) v.ratio[1] = s[1] / top[1];
+      }
+    }
+    return v;
+  };
+
+  int item = blockIdx.x * kCompactWarps + (threadIdx.x >> 5);
+  Move now = prepare(item);
+  for (; item < total; item += stride) {
+    Move next = {0, -1, {1.f, 1.f}};
+    bool prepared = false;
+    if (__any_sync(0xffffffffu, now.to >= 0)) {
+#pragma unroll 1
+      for (int at = 0; at < 32; at += ROWS) {
+        uint4 c[2][STEP];
 #pragma unroll
-      for (int i = 0; i < STEP; ++i) {
-        const int r = half + i * RPW + r0;
+        for (int i = 0; i < STEP; ++i) {
+          const int from = __shfl_sync(0xffffffffu, now.from, at + i * RPW + r0);
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const float s = __shfl_sync(0xffffffffu, now.s[p], r);
-          if (base + r < rows) {
-            if (s != top[p]) c[p][i] = fp8_rescale16(c[p][i], s / top[p]);
-            *reinterpret_cast<uint4*>(a.codes + p * a.plane_bytes + (to * bs + base + r) * D + sub * 16) = c[p][i];
+          for (int p = 0; p < 2; ++p)
+            c[p][i] = __ldcg(reinterpret_cast<const uint4*>(a.codes + p * a.plane_bytes + (size_t)from * D + sub * 16));
+        }
+        if (!prepared) {  // the next item's chain of loads runs beside this one's rows
+          next = prepare(item + stride);
+          prepared = true;
+        }
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) {
+          const int r = at + i * RPW + r0, to = __shfl_sync(0xffffffffu, now.to, r);
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const float ratio = __shfl_sync(0xffffffffu, now.ratio[p], r);
+            if (to >= 0) {
+              if (ratio != 1.f) c[p][i] = fp8_rescale16(c[p][i], ratio);
+              *reinterpret_cast<uint4*>(a.codes + p * a.plane_bytes + (size_t)to * D + sub * 16) = c[p][i];
+            }
           }
         }
       }
     }
+    if (!prepared) next = prepare(item + stride);
+    now = next;
   }
 }
 
@@ -327,20 +378,23 @@ int launch_fp8_evict(const clove_fp8_pool& pool, const Fp8EvictCall& c, cudaStre
   a.num_blocks = pool.num_blocks;
   a.block_size = pool.block_size;
   a.num_kv_heads = pool.num_kv_heads;
-  // CTAs per (sequence, head): parts of at most 8192 tokens of the longest sequence, in a cluster of up to 8.  Keys
-  // that fit stay in shared memory (room for 8192 to 48 K of them); longer parts are read again.
+  // CTAs per (sequence, head): parts of at most 8192 tokens of the longest sequence (of 2048 while the GPU has room
+  // for more CTAs), in a cluster of up to 8.  Short parts alone on a CTA take few threads, so that many fit an SM.
   const int most = std::min(c.budget, c.max_ctx);
+  const long long heads = (long long)c.batch * pool.num_kv_heads;
   int C = 1;
-  while (C < 8 && (long long)C * 8192 < c.max_ctx) C *= 2;
-  const int part = ((c.max_ctx + C - 1) / C + kSelThreads - 1) / kSelThreads * kSelThreads;
-  const int room = part <= kMaxRoom ? part : 0, smem = room * (int)sizeof(uint32_t);
-  int rc = fp8_launch_status("cudaFuncSetAttribute", cudaFuncSetAttribute(fp8_select_kernel,
-                                                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                                          kMaxRoom * (int)sizeof(uint32_t)));
+  while (C < 8 && (C * 8192LL < c.max_ctx || (C * 2048LL < c.max_ctx && 2 * C * heads <= 2 * pool.num_sms))) C *= 2;
+  auto select = C == 1 ? fp8_select_kernel<256, 5> : fp8_select_kernel<512, 3>;
+  const unsigned threads = C == 1 ? 256 : 512;
+  const int part = ((c.max_ctx + C - 1) / C + 511) / 512 * 512;
+  const int room = std::min(part, kMaxRoom), smem = room * (int)sizeof(uint32_t);
+  int rc = fp8_launch_status("cudaFuncSetAttribute",
+                             cudaFuncSetAttribute(select, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                  kMaxRoom * (int)sizeof(uint32_t)));
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(C * pool.num_kv_heads, c.batch);
-  cfg.blockDim = dim3(kSelThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -350,20 +404,25 @@ int launch_fp8_evict(const clove_fp8_pool& pool, const Fp8EvictCall& c, cudaStre
   attr[1].val.clusterDim = {(unsigned)C, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  rc = fp8_launch_status("fp8_evict select launch", cudaLaunchKernelEx(&cfg, fp8_select_kernel, a, C, room));
+  rc = fp8_launch_status("fp8_evict select launch", cudaLaunchKernelEx(&cfg, select, a, C, room));
   if (rc) return rc;
   count_launches(1);
   if (most == 0) return CLOVE_OK;
-  const int blocks = (most + pool.block_size - 1) / pool.block_size;
-  cfg.gridDim = dim3((blocks + kCompactWarps - 1) / kCompactWarps, pool.num_kv_heads, c.batch);
+  const int chunks = (most + 31) / 32;
+  if (heads * chunks > 0x7fffffff - (1 << 20)) {
+    set_last_error("fp8_evict: %lld rows to move", heads * chunks * 32);
+    return CLOVE_ERR_UNSUPPORTED;
+  }
+  cfg.gridDim = dim3((unsigned)std::min<long long>((heads * chunks + kCompactWarps - 1) / kCompactWarps,
+                                                   (long long)pool.num_sms * kCompactPerSm));
   cfg.blockDim = dim3(kCompactWarps * 32);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
   cudaError_t e;
   switch (pool.head_dim) {
-    case 64: e = cudaLaunchKernelEx(&cfg, fp8_compact_kernel<64>, a); break;
-    case 128: e = cudaLaunchKernelEx(&cfg, fp8_compact_kernel<128>, a); break;
-    default: e = cudaLaunchKernelEx(&cfg, fp8_compact_kernel<256>, a); break;
+    case 64: e = cudaLaunchKernelEx(&cfg, fp8_compact_kernel<64>, a, c.batch, chunks); break;
+    case 128: e = cudaLaunchKernelEx(&cfg, fp8_compact_kernel<128>, a, c.batch, chunks); break;
+    default: e = cudaLaunchKernelEx(&cfg, fp8_compact_kernel<256>, a, c.batch, chunks); break;
   }
   count_launches(1);
   return fp8_launch_status("fp8_evict compact launch", e);
