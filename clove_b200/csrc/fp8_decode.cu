@@ -258,7 +258,20 @@ __global__ void __launch_bounds__(32) fp8_append_kernel(const Fp8Args a) {
   fp8_store_new<D>(a, h, L, lane, n);
 }
 
-// Barrier operations and reads by shared-memory address: the producer's
+// Shared-memory reads by address (the compiler would take a generic pointer's
+// longer way).
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+
+// Barrier operations by shared-memory address: the producer's
 // per-stage loop has to stay small.
 __device__ __forceinline__ bool try_wait_at(uint32_t bar, uint32_t parity) {
   uint32_t ok;
@@ -271,6 +284,11 @@ __device__ __forceinline__ bool try_wait_at(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void expect_tx_at(uint32_t bar, uint32_t bytes) {
   asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes)
                : "memory");
@@ -282,12 +300,6 @@ __device__ __forceinline__ void tma_slice(uint32_t dst, const CUtensorMap* map, 
       "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(bar), "l"(policy)
       : "memory");
 }
-__device__ __forceinline__ int lds32(uint32_t a) {
-  int v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
-
 // The bounded wait for a ring slot, out of line.  False: it ran out, or the
 // CTA has given up.
 __device__ __noinline__ bool slot_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int* err, uint32_t limit) {
@@ -304,17 +316,17 @@ __device__ __noinline__ bool slot_wait(uint32_t bar, uint32_t parity, volatile i
 // the CTA's range, posts each piece, appends the new token where the piece
 // ends its sequence, and streams the slices.
 //
-// It must issue a stage every ~700 clocks beside the consumers, so what runs
-// once a stage is short, on one lane (a loop that leaves the instruction
-// cache costs over 1000 clocks here): the warp prepares 32 slices at a time
-// (table entries, copy rows, scales; loaded a group ahead), leaves the rows in
-// `rows` and the scales in the ring `scl`, and lane 0 issues their copies.
+// It must issue a stage every ~1300 clocks beside the consumers, so what runs
+// once a stage is short (a loop that leaves the instruction cache costs over
+// 1000 clocks here): the warp prepares 32 slices at a time (table entries,
+// copy rows, scales; loaded a group ahead), leaves the scales in the ring
+// `scl` and issues the copies.
 // The scales of slice i of stage gs are at scl[(gs * sb + i) % kSclRing]: a
 // group is written when at most nstage stages are unconsumed, so nstage * sb +
 // 32 <= kSclRing entries are live.
 template <typename T, int D>
 __device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* map, const SmemPtrs& sm, const SmemPlan& sp, float2* scl,
-                            int* rows, int sb, const WalkStart& ws) {
+                            int sb, const WalkStart& ws) {
   constexpr int RPT = D >= 128 ? D / 128 : 1;  // rows of the copies' tensor map per token
   const int lane = threadIdx.x & 31, sub_shift = a.real_shift - a.slice_shift;
   const int vs = a.block_size, H = a.num_kv_heads, Hq = H * a.group;
@@ -322,7 +334,7 @@ __device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* map, const Smem
   const uint32_t q_bytes = (uint32_t)(a.group * D * (int)sizeof(T));
   const uint64_t pol = policy_evict_first();
   const uint32_t full = smem_u32(sm.full), empty = smem_u32(sm.empty), ring = smem_u32(sm.ring);
-  const uint32_t rows_at = smem_u32(rows), stage_bytes = (uint32_t)sp.stage_bytes;
+  const uint32_t stage_bytes = (uint32_t)sp.stage_bytes;
   int slot = 0, uk = 0, stage = 0;  // ring slot of the next stage, unit slot, stages issued
   uint32_t phase = 0, uphase = 0;
   bool aborted = false;
@@ -356,6 +368,7 @@ __device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* map, const Smem
   };
 
   const int alpha = a.seg_cost, sb_shift = 31 - __clz(sb);
+
   int b = ws.b, h = ws.h, off = ws.off, npiece = 0;
   int left = (int)(ws.hi - ws.lo);  // stream positions of the range still to walk
   int L = b >= 0 ? clamp_ctx(a.context_lens, b, a.max_ctx, a.append) : 0;
@@ -463,7 +476,7 @@ __device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* map, const Smem
     for (int j0 = 0; j0 == 0 || j0 < x.nblk; j0 += 32) {
       const int n = min(32, x.nblk - j0);  // slices of this group
       const bool final = j0 + 32 >= x.nblk;
-      rows[lane] = cur.row;
+      const int issued = cur.row;
       scl[(stage * sb + lane) & (kSclRing - 1)] = make_float2(cur.sk, cur.sv);
       __syncwarp();
       if (final) {
@@ -472,47 +485,44 @@ __device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* map, const Smem
         cur = resolve(x, j0 + 32, e1);
         if (j0 + 64 < x.nblk) e1 = entry(x, j0 + 64);
       }
-      // lane 0 issues the group; before a piece's last stages the warp sees
-      // to the next piece's loads
+      // issue the group; before a piece's last stages come the next piece's loads
       const int nst = (n + sb - 1) >> sb_shift, cut = final ? (nst + 1) / 2 : nst;
 #pragma unroll 1
       for (int part = 0; part < 2; ++part) {
         const int s0 = part == 0 ? 0 : cut, s1 = part == 0 ? cut : nst;
-        if (lane == 0) {
-          int s = s0;
-          if (first && a.inject_stall && s < s1) {  // test hook: the CTA's first stage is never filled
-            ++s;
-            ++slot;
-          }
-          first = false;
-#pragma unroll 1
-          for (; s < s1; ++s) {
-            if (slot == a.nstage) {
-              slot = 0;
-              phase ^= 1;
-            }
-            if (!try_wait_at(empty + slot * 8, phase ^ 1) && !slot_wait(empty + slot * 8, phase ^ 1, sm.misc, a.err, a.wait_limit)) {
-              ok = 0;
-              break;
-            }
-            const int m = min(sb, n - s * sb);
-            const uint32_t bar = full + slot * 8;
-            expect_tx_at(bar, slice_bytes * (uint32_t)m);
-            uint32_t dst = ring + slot * stage_bytes, src = rows_at + s * sb * 4;
-#pragma unroll 1
-            for (int i = 0; i < m; ++i) {  // one copy per slice: its K tile, then its V tile
-              tma_slice(dst, map, bar, lds32(src), pol);
-              dst += slice_bytes;
-              src += 4;
-            }
-            ++slot;
-          }
+        int s = s0;
+        if (first && a.inject_stall && s < s1) {  // test hook: the CTA's first stage is never filled
+          ++s;
+          ++slot;
         }
-        __syncwarp();
+        first = false;
+#pragma unroll 1
+        for (; s < s1; ++s) {
+          if (slot == a.nstage) {
+            slot = 0;
+            phase ^= 1;
+          }
+          // the whole warp waits and counts, one lane issues: operands stay in uniform registers
+          if (!__all_sync(0xffffffffu, try_wait_at(empty + slot * 8, phase ^ 1)) &&
+              !__all_sync(0xffffffffu, slot_wait(empty + slot * 8, phase ^ 1, sm.misc, a.err, a.wait_limit))) {
+            ok = 0;
+            break;
+          }
+          const int m = min(sb, n - s * sb);
+          const uint32_t bar = full + slot * 8;
+          if (elect_one()) expect_tx_at(bar, slice_bytes * (uint32_t)m);
+          uint32_t dst = ring + slot * stage_bytes;
+#pragma unroll 1
+          for (int i = 0; i < m; ++i) {  // one copy per slice: its K tile, then its V tile
+            const int row = __shfl_sync(0xffffffffu, issued, s * sb + i);
+            if (elect_one()) tma_slice(dst, map, bar, row, pol);
+            dst += slice_bytes;
+          }
+          ++slot;
+        }
         if (part == 0 && final && have2) preload(x2);
       }
       stage += nst;
-      ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
     }
     if (!ok) {
@@ -561,19 +571,6 @@ __device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
-
-// Shared-memory reads by address (the compiler would take a generic pointer's
-// longer way).
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
 }
 
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
@@ -643,19 +640,25 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// tanh: up to kTanhNear the continued fraction x / (1 + x^2 / (3 + x^2 / (5 +
-// ..))) cut after the sixth level (off by less than 2^-27 there), beyond it
-// 1 - 2 / (1 + e^2x).  The library's version, unrolled over a pass, does not
-// fit the instruction cache beside the rest.
-constexpr float kTanhNear = 1.25f;
+// tanh for |x| <= kTanhNear, where scores below a cap mostly are: the series
+// to x^9 (off by less than 2^-24 of the value there).
+constexpr float kTanhNear = 0.3f;
 __device__ __forceinline__ float tanh_near(float x) {
   const float y = x * x;
-  return __fdividef(x * fmaf(y, fmaf(y, 21.f, 1260.f), 10395.f), fmaf(y, fmaf(y, y + 210.f, 4725.f), 10395.f));
+  return fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), x);
 }
-__device__ __forceinline__ float tanh_far(float x) {
-  const float e = ex2(fabsf(x) * (2.f * kLog2e));
-  const float r = copysignf(1.f - __fdividef(2.f, 1.f + e), x);
-  return fabsf(x) > kTanhNear ? r : tanh_near(x);
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// tanh for any x: up to 1.25 the continued fraction x / (1 + x^2 / (3 + x^2 /
+// (5 + ..))) cut after the sixth level (off by less than 2^-27), beyond it 1 -
+// 2 / (1 + e^2x).
+__device__ __forceinline__ float tanh_any(float x) {
+  const float y = x * x, e = ex2(fabsf(x) * (2.f * kLog2e));
+  const float low = x * fmaf(y, fmaf(y, 21.f, 1260.f), 10395.f) * rcp(fmaf(y, fmaf(y, y + 210.f, 4725.f), 10395.f));
+  return fabsf(x) > 1.25f ? copysignf(fmaf(-2.f, rcp(1.f + e), 1.f), x) : low;
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -701,7 +704,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
   fp8_prologue<D>(a, &walk);
 
   if (warp == 0) {
-    fp8_produce<T, D>(a, &map, sm, sp, scl, reinterpret_cast<int*>(scl + kSclRing), sb, walk);
+    fp8_produce<T, D>(a, &map, sm, sp, scl, sb, walk);
     return;
   }
 
@@ -856,7 +859,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
 #pragma unroll
               for (int e = 0; e < NE; ++e)
 #pragma unroll
-                for (int c = 0; c < 2; ++c) z[e][c] = tanh_far(z[e][c]) * cap;
+                for (int c = 0; c < 2; ++c) z[e][c] = tanh_any(z[e][c]) * cap;
             } else {
 #pragma unroll
               for (int e = 0; e < NE; ++e)
@@ -1223,7 +1226,7 @@ static int fp8_cfg(const clove_fp8_pool& pool, int slice, int group, Fp8Cfg* out
   Fp8Cfg c;
   const int stage = smem_plan(slice, D, 1, sb, 1, scratch, qb, 1).stage_bytes;
   auto bytes = [&](int n) {
-    return smem_plan(slice, D, 1, sb, n, scratch, qb, 1).total + kSclRing * (int)sizeof(float2) + 32 * (int)sizeof(int) + 1024;
+    return smem_plan(slice, D, 1, sb, n, scratch, qb, 1).total + kSclRing * (int)sizeof(float2) + 1024;
   };
   // as deep a ring as two CTAs on an SM leave room for
   c.nstage = std::max(1, ring / stage / kFp8Warps) * kFp8Warps;
