@@ -106,31 +106,40 @@ __device__ void fp8_prologue(const Fp8Args& a, WalkStart* out) {
     return;
   }
   __shared__ int warp_tot[32];
-  __shared__ long long s_sum;
+  __shared__ long long s_rest;
   __shared__ int s_found;
   const int row_floats = H * a.group * D;
   if (tid == 0) {
-    s_sum = 0;
+    s_rest = 0;
     s_found = 0;
   }
-  __syncthreads();
-  long long mine = 0;
-  for (int b = tid; b < a.batch; b += nt) {
-    const int raw = __ldg(a.context_lens + b);
+  // stream positions of each of sequence b's segments; empty sequences get their zero rows on the way
+  auto length = [&](int b, bool first_look) {
+    if (b >= a.batch) return 0;
     const int L = clamp_ctx(a.context_lens, b, a.max_ctx, a.append);
-    if (blockIdx.x == 0 && raw != L - a.append) atomicOr(a.err, CLOVE_FLAG_CTX_RANGE);
-    if (L > 0) mine += num_slices(a, L) + a.seg_cost;
-    if (L == 0 && b % a.num_ctas == (int)blockIdx.x) {
-      float4* row = reinterpret_cast<float4*>(a.out + (size_t)b * row_floats);
-      for (int i = 0; i < row_floats / 4; ++i) row[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (first_look) {
+      if (blockIdx.x == 0 && __ldg(a.context_lens + b) != L - a.append) atomicOr(a.err, CLOVE_FLAG_CTX_RANGE);
+      if (L == 0 && b % a.num_ctas == (int)blockIdx.x) {
+        float4* row = reinterpret_cast<float4*>(a.out + (size_t)b * row_floats);
+        for (int i = 0; i < row_floats / 4; ++i) row[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
     }
-  }
+    return L > 0 ? num_slices(a, L) + a.seg_cost : 0;
+  };
+  // the first nt sequences by a scan (usually all of them), the sum of the others
+  int len = length(tid, true), tot;
+  int excl = block_excl_scan(len, warp_tot, &tot);
+  if (a.batch > nt) {
+    long long mine = 0;
+#pragma unroll 1
+    for (int b = tid + nt; b < a.batch; b += nt) mine += length(b, true);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0 && mine) atomicAdd(reinterpret_cast<unsigned long long*>(&s_sum), (unsigned long long)mine);
-  __syncthreads();
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0 && mine) atomicAdd(reinterpret_cast<unsigned long long*>(&s_rest), (unsigned long long)mine);
+    __syncthreads();
+  }
   // floor(c W / P) = c (W / P) + floor(c (W mod P) / P), the last in 32 bits
-  const unsigned long long W = (unsigned long long)s_sum * H, quot = udiv64(W, a.num_ctas);
+  const unsigned long long W = (unsigned long long)(s_rest + tot) * H, quot = udiv64(W, a.num_ctas);
   const unsigned rest = (unsigned)(W - quot * a.num_ctas), c = blockIdx.x;
   const long long lo = (long long)(c * quot + c * rest / a.num_ctas);
   const long long hi = (long long)((c + 1) * quot + (c + 1) * rest / a.num_ctas);
@@ -142,25 +151,25 @@ __device__ void fp8_prologue(const Fp8Args& a, WalkStart* out) {
     out->off = 0;
     if (blockIdx.x == 0) *a.total = (long long)W;
   }
+  __syncthreads();
   if (lo < hi) {
     long long carry = 0;
-    for (int base = 0; base < a.batch; base += nt) {
-      const int b = base + tid;
-      const int L = b < a.batch ? clamp_ctx(a.context_lens, b, a.max_ctx, a.append) : 0;
-      const int len = L > 0 ? num_slices(a, L) + a.seg_cost : 0;
-      int tot;
-      const int excl = block_excl_scan(len, warp_tot, &tot);
+#pragma unroll 1
+    for (int base = 0;; ) {
       const long long s0 = (carry + excl) * H;
       if (len > 0 && s0 <= lo && lo < s0 + (long long)len * H) {
         const unsigned long long r = lo - s0, hh = udiv64(r, len);
-        out->b = b;
+        out->b = base + tid;
         out->h = (int)hh;
         out->off = (int)(r - hh * len);
         s_found = 1;
       }
       carry += tot;
+      base += nt;
       __syncthreads();
-      if (s_found) break;
+      if (s_found || base >= a.batch) break;
+      len = length(base + tid, false);
+      excl = block_excl_scan(len, warp_tot, &tot);
     }
   }
   __syncthreads();
@@ -1085,31 +1094,49 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
 // ---------------------------------------------------------------------------
 // weights: mass += sum over the group of 2^(z - M) / L
 // ---------------------------------------------------------------------------
-constexpr int kMassThreads = 256, kMassTokens = 1024;
+constexpr int kMassThreads = 256, kMassTokens = 128;  // tokens per warp and item: four per lane
 
+// Items (sequence, KV head, 128 tokens), one warp each; those behind a
+// sequence's end cost a look at its length.
 __global__ void __launch_bounds__(kMassThreads) fp8_mass_kernel(const Fp8Args a) {
-  const int b = blockIdx.z, h = blockIdx.y, H = a.num_kv_heads, G = a.group, bs = a.real_block;
+  const int H = a.num_kv_heads, G = a.group, bs = a.real_block, lane = threadIdx.x & 31;
+  const int chunks = (a.max_ctx + kMassTokens - 1) / kMassTokens;
+  const long long total = (long long)a.batch * H * chunks;
   griddep_wait();
-  const int L = clamp_ctx(a.context_lens, b, a.max_ctx, a.append);
-  const int t0 = a.window > 0 ? max(0, L - a.window) : 0;
-  const int from = max(t0, (int)blockIdx.x * kMassTokens), to = min(L, ((int)blockIdx.x + 1) * kMassTokens);
-  if (from >= to) return;
-  const size_t row = (size_t)b * H * G + (size_t)h * G;
-  for (int t = from + threadIdx.x; t < to; t += kMassThreads) {
-    int blk = __ldg(a.block_tables + (size_t)b * a.bt_stride + t / bs);
-    const bool mine = a.append && t == L - 1;
-    if (blk < 0 || blk >= a.num_blocks) {
-      if (mine) continue;  // the token was not written
-      blk = 0;
-    }
-    float w = 0.f;
-#pragma unroll 8
-    for (int g = 0; g < G; ++g) {
-      const float2 st = __ldg(a.row_state + row + g);
-      w = fmaf(exp2f(__ldcs(a.z + (row + g) * a.z_stride + t) - st.x), st.y, w);
-    }
+  for (long long i = (long long)blockIdx.x * (kMassThreads / 32) + (threadIdx.x >> 5); i < total;
+       i += (long long)gridDim.x * (kMassThreads / 32)) {
+    const int head = (int)(i / chunks), b = head / H, h = head - b * H;
+    const int L = clamp_ctx(a.context_lens, b, a.max_ctx, a.append);
+    const int t0 = a.window > 0 ? max(0, L - a.window) : 0;
+    const int t = (int)(i - (long long)head * chunks) * kMassTokens + 4 * lane;  // this lane's first token
+    if (t >= L || t + 4 <= t0) continue;
+    int blk = __ldg(a.block_tables + (size_t)b * a.bt_stride + (t >> a.real_shift));
+    const bool bad = blk < 0 || blk >= a.num_blocks;
+    if (bad) blk = 0;
     float* dst = a.mass + ((size_t)blk * H + h) * bs + (t & (bs - 1));
-    *dst = mine ? w : *dst + w;
+    const float4 was = *reinterpret_cast<const float4*>(dst);
+    float w[4] = {0.f, 0.f, 0.f, 0.f};
+    const float* z = a.z + (size_t)head * G * a.z_stride + t;
+#pragma unroll 4
+    for (int g = 0; g < G; ++g) {
+      const float2 st = __ldg(a.row_state + (size_t)head * G + g);
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(z + (size_t)g * a.z_stride));
+      w[0] = fmaf(ex2(v.x - st.x), st.y, w[0]);
+      w[1] = fmaf(ex2(v.y - st.x), st.y, w[1]);
+      w[2] = fmaf(ex2(v.z - st.x), st.y, w[2]);
+      w[3] = fmaf(ex2(v.w - st.x), st.y, w[3]);
+    }
+    if (t >= t0 && t + 4 <= L - a.append) {
+      *reinterpret_cast<float4*>(dst) = make_float4(was.x + w[0], was.y + w[1], was.z + w[2], was.w + w[3]);
+    } else {
+      const float old[4] = {was.x, was.y, was.z, was.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (t + k < t0 || t + k >= L) continue;
+        const bool mine = a.append && t + k == L - 1;  // the new token starts at its own weight
+        if (!(mine && bad)) dst[k] = mine ? w[k] : old[k] + w[k];
+      }
+    }
   }
 }
 
@@ -1117,6 +1144,7 @@ __global__ void __launch_bounds__(kMassThreads) fp8_mass_kernel(const Fp8Args a)
 // host side
 // ---------------------------------------------------------------------------
 constexpr int kFp8Warps = 3;
+constexpr int kDirectTokens = 1024;
 constexpr int kFp8Ring = 96 * 1024;
 constexpr int kFp8Smem = 227 * 1024 / 2 - 1024;  // of each of two CTAs on an SM
 
@@ -1281,7 +1309,8 @@ static int run_fp8(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) 
     count_launches(1);
   }
   if (a.z != nullptr) {
-    const dim3 grid((a.max_ctx + kMassTokens - 1) / kMassTokens, a.num_kv_heads, a.batch);
+    const long long items = (long long)a.batch * a.num_kv_heads * ((a.max_ctx + kMassTokens - 1) / kMassTokens);
+    const dim3 grid((unsigned)std::min(items / (kMassThreads / 32) + 1, 8LL * pool.num_sms));
     rc = fp8_launch_status("fp8_decode weights launch", launch_chained(fp8_mass_kernel, grid, kMassThreads, 0, stream, a));
     if (rc) return rc;
     count_launches(1);
@@ -1346,7 +1375,12 @@ int launch_fp8_decode(const clove_fp8_pool& pool, const Fp8DecodeCall& c, cudaSt
     a.z = reinterpret_cast<float*>(ws + L.off_z);
     a.z_stride = L.z_stride;
   }
-  a.direct = 0;
+  // Few and short sequences, each KV head whole on one CTA: no partition to work out and nothing to combine.
+  // Measured with 8 heads: 1 sequence of 100 / 1000 / 2000 tokens 9.4 / 16.5 / 22.6 us against 20.5 / 19.2 / 20.5 split;
+  // 64 sequences (512 heads) of 100 / 1000: 18.5 / 37.1 against 22.3 / 40.0; 128 of 100 / 1000: 32.9 / 71.6 against
+  // 28.8 / 60.8, since the CTAs then come in more than two waves.
+  const int longest = c.scores.window > 0 ? std::min(c.scores.window, c.max_ctx) : c.max_ctx;
+  a.direct = (long long)c.batch * pool.num_kv_heads <= 4LL * pool.num_sms && longest <= kDirectTokens;
   a.append_here = a.append && (a.direct || slice == pool.block_size);
   switch (c.dtype) {
     case CLOVE_DTYPE_F32: return run_fp8_dim<float>(pool, a, stream);
