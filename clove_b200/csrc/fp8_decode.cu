@@ -16,11 +16,12 @@
 //     row is scaled to the top of the f16 range (bf16 elements 2^-31 below the
 //     row's largest lose bits), an f32 query the sum of two halves and so two
 //     MMAs;
-//   - a weight is the sum of two halves.  In P.V the queries are the MMA's
-//     rows, at most 8 of 16: the high halves are rows 0..7, the low halves
-//     rows 8..15 of the same instruction, and the two results meet in one
-//     thread's registers.  An 8x8 transpose of f16 pairs (movmatrix) turns the
-//     score fragment into that operand;
+//   - a weight is the sum of two halves, and the value sum is transposed too:
+//     V^T (16 dims) times P^T (8 queries).  With up to 4 queries columns 4..7
+//     repeat queries 0..3, and one MMA takes the high halves in columns 0..3
+//     and the low halves in 4..7 (their sums meet once a piece); with more,
+//     each half has its MMA.  An 8x8 transpose of f16 pairs (movmatrix) turns
+//     the score fragment into that operand;
 //   - weights are 2^(z - m + 14): the f16 range below the largest weight is 14
 //     binades longer than with 2^(z - m), so a weight is off by at most 2^-39
 //     of the row's largest however many light tokens there are;
@@ -682,9 +683,10 @@ __device__ __forceinline__ float floor_pow2(float x) {
 }
 __device__ __forceinline__ float inv_pow2(float x) { return __int_as_float((254 << 23) - __float_as_int(x)); }
 
-// kExtra: scores may be capped, biased or kept (the plain variant has none of
-// that code: what a pass runs has to fit the instruction cache).
-template <typename T, int D, int NCW, bool kExtra>
+// kExtra: scores may be capped, biased or kept; kTwin: groups of up to 4
+// queries.  (A variant has none of the others' code: what a pass runs has to
+// fit the instruction cache.)
+template <typename T, int D, int NCW, bool kExtra, bool kTwin>
 __global__ void __launch_bounds__((NCW + 1) * 32, 2)
     fp8_decode_kernel(const __grid_constant__ CUtensorMap map, const Fp8Args a) {
   static_assert(NCW == 3, "the hand-off sums three warps' states");
@@ -692,7 +694,6 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
   constexpr int KJ = D / 64;                   // 16-byte K chunks per lane and token
   constexpr int VH = D >= 128 ? D / 128 : 1;   // 128-byte rows per token
   constexpr int VP = D >= 128 ? 2 : 1;         // 8-byte V units per lane and row
-  constexpr int NT = D / 8;                    // n-tiles of the value sum
   constexpr int S = state_stride(D);
   constexpr int PT = D == 256 ? 32 : 64;       // tokens per pass
   constexpr int NG = PT / 16, NE = PT / 8;     // MMA steps and 8-token tiles of a pass
@@ -719,6 +720,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
 
   const int cw = warp - 1, g = lane >> 2, tq = lane & 3;
   const int vshift = a.slice_shift;
+  const int gq = kTwin ? g & 3 : g;  // kTwin: columns 4..7 repeat queries 0..3
   // Read offsets within a pass: K rows g (+ 8 e), V rows 2 tq + (i & 1) (+ 8 n);
   // the swizzle's row bits do not change with the multiples of 8 tokens.
   uint32_t koff[KJ], voff[2][VH * VP];
@@ -746,7 +748,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
     const int j_first = ((cw - gbase) % NCW + NCW) % NCW;
     const bool mine = j_first < x.nstages;
     if (mine) {
-      const uint32_t qaddr = smem_u32(sm.qbuf + uk * sp.q_stride) + g * D * (int)sizeof(T);
+      const uint32_t qaddr = smem_u32(sm.qbuf + uk * sp.q_stride) + gq * D * (int)sizeof(T);
       float q[KJ * 16];
       float amax = 0.f;
 #pragma unroll
@@ -754,7 +756,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
 #pragma unroll
         for (int i = 0; i < 16; i += 16 / (int)sizeof(T)) {
           uint4 w = make_uint4(0, 0, 0, 0);
-          if (g < group) w = lds128(qaddr + (k_chunk<D>(tq, j) * 16 + i) * (int)sizeof(T));
+          if (gq < group) w = lds128(qaddr + (k_chunk<D>(tq, j) * 16 + i) * (int)sizeof(T));
           unpack16<T>(w, q + j * 16 + i);
         }
 #pragma unroll
@@ -766,7 +768,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
       float f = a.scale * __int_as_float((127 + max(e, -126)) << 23);
       if (e < -126) f *= 0.5f;
       f = kExtra && a.softcap > 0.f ? f / a.softcap : f * kLog2e;
-      const float s = kExtra && a.slopes != nullptr && g < group ? __ldg(a.slopes + x.h * group + g) * kLog2e : 0.f;
+      const float s = kExtra && a.slopes != nullptr && gq < group ? __ldg(a.slopes + x.h * group + gq) * kLog2e : 0.f;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         zf[c] = __shfl_sync(0xffffffffu, f, (2 * tq + c) * 4);
@@ -793,9 +795,10 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
                       : nullptr;
 
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, vref = 0.f;
-    float o[NT][2];
+    // value sums: o[8 i + 2 k + c] is dim k (of 4) of half i of this lane's V units, query 2 tq + c
+    float o[D / 4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = 0.f;
+    for (int n = 0; n < D / 4; ++n) o[n] = 0.f;
 
     bool aborted = false;
     for (int j = j_first; j < x.nstages; j += NCW) {
@@ -920,23 +923,22 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
           m[c] = mn;
           l[c] *= corr[c];
         }
-        // the P operand: high halves in rows 0..7, low halves in rows 8..15
-        uint32_t pa[NG][4];
+        // the P^T operand (tokens x queries): both halves of the weights, or, where columns 4..7 repeat the queries,
+        // the high halves in columns 0..3 and the low ones in 4..7
+        uint32_t ph[NE], pl[kTwin ? 1 : NE];
 #pragma unroll
         for (int e = 0; e < NE; ++e) {
           const float p0e = ex2(z[e][0] - ms[0]), p1e = ex2(z[e][1] - ms[1]), f = wv[e] * vinv;
           l[0] += p0e;
           l[1] += p1e;
-          uint32_t ph, pl;
-          split_halves(p0e * f, p1e * f, ph, pl);
-          pa[e >> 1][2 * (e & 1)] = transpose8x8(ph);
-          pa[e >> 1][2 * (e & 1) + 1] = transpose8x8(pl);
+          uint32_t hi2, lo2;
+          split_halves(p0e * f, p1e * f, hi2, lo2);
+          ph[e] = transpose8x8(kTwin && tq >= 2 ? lo2 : hi2);
+          if constexpr (!kTwin) pl[e] = transpose8x8(lo2);
         }
-        // the value sum's rows are queries g: their correction is held by lanes tq = g / 2
-        const float c0 = __shfl_sync(0xffffffffu, corr[0], g >> 1), c1 = __shfl_sync(0xffffffffu, corr[1], g >> 1);
-        const float oc = (g & 1 ? c1 : c0) * (vref * vinv);
+        const float oc[2] = {corr[0] * (vref * vinv), corr[1] * (vref * vinv)};
         vref = vnew;
-        // ---- value sum ----
+        // ---- value sum, V^T (16 dims) times P^T (8 queries) ----
 #pragma unroll
         for (int u = 0; u < VH * VP; ++u) {
           uint2 vw[NG][4];  // tokens 16 k + 2 tq + {0, 1, 8, 9}, 8 dims each
@@ -947,30 +949,36 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
               vw[k][i] = lds64(vbase + voff[i & 1][u] + tile_at(p0 + 16 * k + 8 * (i >> 1)));
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            float d[4][4];
+            float d[2][4];  // MMA i: rows g and g + 8 are this lane's dims 2 i and 2 i + 1 of the four
 #pragma unroll
             for (int k = 0; k < NG; ++k) {
               const uint32_t t0 = w ? vw[k][0].y : vw[k][0].x, t1 = w ? vw[k][1].y : vw[k][1].x;
               const uint32_t t2 = w ? vw[k][2].y : vw[k][2].x, t3 = w ? vw[k][3].y : vw[k][3].x;
-              uint32_t b0[4], b1[4];  // token pairs of dims 0..3
-              codes4(__byte_perm(t0, t1, 0x5140), b0[0], b0[1]);
-              codes4(__byte_perm(t0, t1, 0x7362), b0[2], b0[3]);
-              codes4(__byte_perm(t2, t3, 0x5140), b1[0], b1[1]);
-              codes4(__byte_perm(t2, t3, 0x7362), b1[2], b1[3]);
+              uint32_t v0[4], v1[4];  // token pairs of dims 0..3
+              codes4(__byte_perm(t0, t1, 0x5140), v0[0], v0[1]);
+              codes4(__byte_perm(t0, t1, 0x7362), v0[2], v0[3]);
+              codes4(__byte_perm(t2, t3, 0x5140), v1[0], v1[1]);
+              codes4(__byte_perm(t2, t3, 0x7362), v1[2], v1[3]);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
+              for (int i = 0; i < 2; ++i) {
                 if (k == 0)
-                  mma_f16_first(d[i], pa[0][0], pa[0][1], pa[0][2], pa[0][3], b0[i], b1[i]);
+                  mma_f16_first(d[i], v0[2 * i], v0[2 * i + 1], v1[2 * i], v1[2 * i + 1], ph[0], ph[1]);
                 else
-                  mma_f16(d[i], pa[k][0], pa[k][1], pa[k][2], pa[k][3], b0[i], b1[i]);
+                  mma_f16(d[i], v0[2 * i], v0[2 * i + 1], v1[2 * i], v1[2 * i + 1], ph[2 * k], ph[2 * k + 1]);
+              }
+              if constexpr (!kTwin) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                  mma_f16(d[i], v0[2 * i], v0[2 * i + 1], v1[2 * i], v1[2 * i + 1], pl[2 * k], pl[2 * k + 1]);
               }
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float* on = o[u * 8 + w * 4 + i];
-              on[0] = fmaf(on[0], oc, d[i][0] + d[i][2]);
-              on[1] = fmaf(on[1], oc, d[i][1] + d[i][3]);
-            }
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                float& on = o[(u * 2 + w) * 8 + 4 * i + r];
+                on = fmaf(on, oc[r & 1], d[i][r]);
+              }
           }
         }
       }
@@ -982,11 +990,18 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
     gbase += x.nstages;
 
     // ---- hand-off: the last warp to finish a piece merges the others' states
-    // (acc, m - 14, l), left in scratch, with its own, still in registers ----
+    // (acc, m - 14, l), left in scratch, with its own, still in registers.
+    // Lane (g, tq) holds queries 2 tq and 2 tq + 1 of its V units' dims. ----
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int s = 4; s < 32; s <<= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], s);
+    if constexpr (kTwin) {  // high and low halves' sums
+#pragma unroll
+      for (int n = 0; n < D / 4; ++n) o[n] += __shfl_xor_sync(0xffffffffu, o[n], 2);
+    }
+#pragma unroll
+    for (int n = 0; n < D / 4; ++n) o[n] *= vref;
     const uint32_t par = (uint32_t)n_done & 1u;
     if (!wait_or_abort(a, sm, &sm.scr_empty[0], par ^ 1u)) return;
     int order = 0;
@@ -996,41 +1011,34 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
     }
     order = __shfl_sync(0xffffffffu, order, 0);
     if (order < NCW - 1) {
-      float* scr = sm.scratch + (size_t)order * group * S;
-      if (g < group && mine) {
-        // thread (g, tq) holds columns 2 tq and 2 tq + 1 of every n-tile
-        float* row = scr + (size_t)g * S;
 #pragma unroll
-        for (int u = 0; u < VH * VP; ++u)
+      for (int c = 0; c < 2; ++c) {
+        if (2 * tq + c >= group) continue;
+        float* row = sm.scratch + ((size_t)order * group + 2 * tq + c) * S;
+        if (mine) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; i += 4)
-              *reinterpret_cast<float4*>(row + (u / VP) * 128 + v_unit<D>(2 * tq + c, u % VP) * 8 + i) =
-                  make_float4(o[u * 8 + i][c] * vref, o[u * 8 + i + 1][c] * vref, o[u * 8 + i + 2][c] * vref,
-                              o[u * 8 + i + 3][c] * vref);
-      }
-      if (g == 0) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          if (2 * tq + c < group) {
-            scr[(size_t)(2 * tq + c) * S + D] = m[c] - 14.f;
-            scr[(size_t)(2 * tq + c) * S + D + 1] = l[c];
-            scr[(size_t)(2 * tq + c) * S + D + 2] = (float)cw;
-          }
+          for (int i = 0; i < VH * VP * 2; ++i)
+            *reinterpret_cast<float4*>(row + (i / (2 * VP)) * 128 + v_unit<D>(g, (i >> 1) % VP) * 8 + (i & 1) * 4) =
+                make_float4(o[8 * i + c], o[8 * i + 2 + c], o[8 * i + 4 + c], o[8 * i + 6 + c]);
+        }
+        if (g == 0) {
+          row[D] = m[c] - 14.f;
+          row[D + 1] = l[c];
+          row[D + 2] = (float)cw;
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.scr_empty[1]);  // [1]: the others' states are in scratch
     } else {
       if (!wait_or_abort(a, sm, &sm.scr_empty[1], par)) return;
-      // row g: this warp's m and l from the lanes that hold them, the others' from scratch
-      const float m0 = __shfl_sync(0xffffffffu, m[0], g >> 1), m1 = __shfl_sync(0xffffffffu, m[1], g >> 1);
-      const float l0 = __shfl_sync(0xffffffffu, l[0], g >> 1), l1 = __shfl_sync(0xffffffffu, l[1], g >> 1);
-      if (g < group) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int q = 2 * tq + c;
+        if (q >= group) continue;
         // Which warp comes last differs from run to run, the sums must not:
         // they are (warp 0 + warp 1) + warp 2, A and B being the others' states
         // in the order of their warps.
-        const float* A = sm.scratch + (size_t)g * S;
+        const float* A = sm.scratch + (size_t)q * S;
         const float* B = A + (size_t)group * S;
         if (A[D + 2] > B[D + 2]) {
           const float* swap = A;
@@ -1043,32 +1051,27 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
           const float po = __fmul_rn(wo, xo), pb = __fmul_rn(wb, xb);
           return __fadd_rn(__fadd_rn(own_last ? pb : po, __fmul_rn(wa, xa)), own_last ? po : pb);
         };
-        const float mo = (g & 1 ? m1 : m0) - 14.f, M = fmaxf(mo, fmaxf(A[D], B[D]));
+        const float mo = m[c] - 14.f, M = fmaxf(mo, fmaxf(A[D], B[D]));
         const float fo = mo == -INFINITY ? 0.f : ex2(mo - M);
         const float fa = A[D] == -INFINITY ? 0.f : ex2(A[D] - M), fb = B[D] == -INFINITY ? 0.f : ex2(B[D] - M);
-        const float L = add(fo, g & 1 ? l1 : l0, fa, A[D + 1], fb, B[D + 1]);
+        const float L = add(fo, l[c], fa, A[D + 1], fb, B[D + 1]);
         const float inv = 1.f / L, norm = x.complete ? inv : 1.f;
-        const int Hq = a.num_kv_heads * group, hq = x.h * group + g;
+        const int Hq = a.num_kv_heads * group, hq = x.h * group + q;
         float* dst = x.complete ? a.out + ((size_t)x.b * Hq + hq) * D
-                                : a.partials + (((size_t)blockIdx.x * 2 + x.slot) * group + g) * S;
+                                : a.partials + (((size_t)blockIdx.x * 2 + x.slot) * group + q) * S;
 #pragma unroll
-        for (int u = 0; u < VH * VP; ++u)
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; i += 4) {
-              const int d = (u / VP) * 128 + v_unit<D>(2 * tq + c, u % VP) * 8 + i;
-              // (a warp without a stage of the piece leaves no acc)
-              float4 va = make_float4(0.f, 0.f, 0.f, 0.f), vb = va;
-              if (fa > 0.f) va = *reinterpret_cast<const float4*>(A + d);
-              if (fb > 0.f) vb = *reinterpret_cast<const float4*>(B + d);
-              *reinterpret_cast<float4*>(dst + d) =
-                  make_float4(add(fo, __fmul_rn(o[u * 8 + i][c], vref), fa, va.x, fb, vb.x) * norm,
-                              add(fo, __fmul_rn(o[u * 8 + i + 1][c], vref), fa, va.y, fb, vb.y) * norm,
-                              add(fo, __fmul_rn(o[u * 8 + i + 2][c], vref), fa, va.z, fb, vb.z) * norm,
-                              add(fo, __fmul_rn(o[u * 8 + i + 3][c], vref), fa, va.w, fb, vb.w) * norm);
-            }
-        if (tq == 0) {
+        for (int i = 0; i < VH * VP * 2; ++i) {
+          const int d = (i / (2 * VP)) * 128 + v_unit<D>(g, (i >> 1) % VP) * 8 + (i & 1) * 4;
+          // (a warp without a stage of the piece leaves no acc)
+          float4 va = make_float4(0.f, 0.f, 0.f, 0.f), vb = va;
+          if (fa > 0.f) va = *reinterpret_cast<const float4*>(A + d);
+          if (fb > 0.f) vb = *reinterpret_cast<const float4*>(B + d);
+          *reinterpret_cast<float4*>(dst + d) = make_float4(add(fo, o[8 * i + c], fa, va.x, fb, vb.x) * norm,
+                                                            add(fo, o[8 * i + 2 + c], fa, va.y, fb, vb.y) * norm,
+                                                            add(fo, o[8 * i + 4 + c], fa, va.z, fb, vb.z) * norm,
+                                                            add(fo, o[8 * i + 6 + c], fa, va.w, fb, vb.w) * norm);
+        }
+        if (g == 0) {
           if (!x.complete) {
             dst[D] = M;
             dst[D + 1] = L;
@@ -1180,7 +1183,18 @@ static Fp8Layout fp8_layout(const clove_fp8_pool& pool, int batch, int num_q_hea
   return L;
 }
 
+// Few and short sequences, each KV head whole on one CTA: no partition to work
+// out and nothing to combine.  Measured with 8 heads of 128, blocks of 16, in
+// us against the split: 1 sequence of 100 / 1000 / 2000 tokens 9.4 / 16.5 /
+// 22.6 against 20.5 / 19.2 / 20.5; 64 sequences (512 heads) of 100 / 1000:
+// 18.5 / 37.1 against 22.3 / 40.0; 128 of 100 / 1000: 32.9 / 71.6 against 28.8
+// / 60.8, since the CTAs then come in more than two waves.
+static bool fp8_direct(const clove_fp8_pool& pool, int batch, int longest) {
+  return (long long)batch * pool.num_kv_heads <= 4LL * pool.num_sms && longest <= kDirectTokens;
+}
+
 size_t fp8_decode_workspace(const clove_fp8_pool& pool, int batch, int num_q_heads, int max_ctx, int accumulate) {
+  if (!accumulate && fp8_direct(pool, batch, max_ctx)) return 0;
   return fp8_layout(pool, batch, num_q_heads, max_ctx, accumulate).total;
 }
 
@@ -1231,12 +1245,12 @@ struct Fp8Cfg {
   int nstage, smem, ctas;
 };
 
-template <typename T, int D, bool kExtra>
+template <typename T, int D, bool kExtra, bool kTwin>
 static int fp8_cfg(const clove_fp8_pool& pool, int slice, int group, Fp8Cfg* out) {
   static std::mutex mu;
   static std::unordered_map<long long, Fp8Cfg> cache;
   static std::unordered_map<int, int> attr;  // device -> shared memory the kernel may use there
-  auto kern = fp8_decode_kernel<T, D, kFp8Warps, kExtra>;
+  auto kern = fp8_decode_kernel<T, D, kFp8Warps, kExtra, kTwin>;
   const long long key = ((long long)pool.device << 32) | ((long long)slice << 8) | group;
   std::lock_guard<std::mutex> lk(mu);
   auto it = cache.find(key);
@@ -1277,11 +1291,11 @@ static int fp8_cfg(const clove_fp8_pool& pool, int slice, int group, Fp8Cfg* out
   return CLOVE_OK;
 }
 
-template <typename T, int D, bool kExtra>
+template <typename T, int D, bool kExtra, bool kTwin>
 static int run_fp8(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) {
   a.stage_blocks = stage_tokens(D) / a.block_size;
   Fp8Cfg c;
-  int rc = fp8_cfg<T, D, kExtra>(pool, a.block_size, a.group, &c);
+  int rc = fp8_cfg<T, D, kExtra, kTwin>(pool, a.block_size, a.group, &c);
   if (rc) return rc;
   a.nstage = c.nstage;
   a.ncw = kFp8Warps;
@@ -1297,7 +1311,7 @@ static int run_fp8(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) 
     count_launches(1);
   }
   rc = fp8_launch_status("fp8_decode launch",
-                         launch_chained(fp8_decode_kernel<T, D, kFp8Warps, kExtra>, dim3(a.num_ctas), (kFp8Warps + 1) * 32,
+                         launch_chained(fp8_decode_kernel<T, D, kFp8Warps, kExtra, kTwin>, dim3(a.num_ctas), (kFp8Warps + 1) * 32,
                                         c.smem, stream, pool.map, a));
   if (rc) return rc;
   count_launches(1);
@@ -1321,7 +1335,8 @@ static int run_fp8(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) 
 template <typename T, int D>
 static int run_fp8_scores(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) {
   const bool extra = a.softcap > 0.f || a.slopes != nullptr || a.z != nullptr;
-  return extra ? run_fp8<T, D, true>(pool, a, stream) : run_fp8<T, D, false>(pool, a, stream);
+  if (a.group <= 4) return extra ? run_fp8<T, D, true, true>(pool, a, stream) : run_fp8<T, D, false, true>(pool, a, stream);
+  return extra ? run_fp8<T, D, true, false>(pool, a, stream) : run_fp8<T, D, false, false>(pool, a, stream);
 }
 
 template <typename T>
@@ -1375,12 +1390,7 @@ int launch_fp8_decode(const clove_fp8_pool& pool, const Fp8DecodeCall& c, cudaSt
     a.z = reinterpret_cast<float*>(ws + L.off_z);
     a.z_stride = L.z_stride;
   }
-  // Few and short sequences, each KV head whole on one CTA: no partition to work out and nothing to combine.
-  // Measured with 8 heads: 1 sequence of 100 / 1000 / 2000 tokens 9.4 / 16.5 / 22.6 us against 20.5 / 19.2 / 20.5 split;
-  // 64 sequences (512 heads) of 100 / 1000: 18.5 / 37.1 against 22.3 / 40.0; 128 of 100 / 1000: 32.9 / 71.6 against
-  // 28.8 / 60.8, since the CTAs then come in more than two waves.
-  const int longest = c.scores.window > 0 ? std::min(c.scores.window, c.max_ctx) : c.max_ctx;
-  a.direct = (long long)c.batch * pool.num_kv_heads <= 4LL * pool.num_sms && longest <= kDirectTokens;
+  a.direct = fp8_direct(pool, c.batch, c.scores.window > 0 ? std::min(c.scores.window, c.max_ctx) : c.max_ctx);
   a.append_here = a.append && (a.direct || slice == pool.block_size);
   switch (c.dtype) {
     case CLOVE_DTYPE_F32: return run_fp8_dim<float>(pool, a, stream);

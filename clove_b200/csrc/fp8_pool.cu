@@ -22,13 +22,16 @@ int cuda_fail(const char* what, cudaError_t e) {
 // Calls may come from any thread with any device current.
 struct OnDevice {
   int prev = -1;
-  bool ok = true;
+  bool ok = true, changed = false;
   explicit OnDevice(int dev) {
     if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-    if (prev != dev) ok = cudaSetDevice(dev) == cudaSuccess;
+    if (prev != dev) {
+      changed = true;
+      ok = cudaSetDevice(dev) == cudaSuccess;
+    }
   }
   ~OnDevice() {
-    if (prev >= 0) cudaSetDevice(prev);
+    if (changed && prev >= 0) cudaSetDevice(prev);
   }
 };
 
@@ -72,19 +75,17 @@ bool known_dtype(int dtype) {
 int finish_pool(clove_fp8_pool* p) {
   cudaError_t e = cudaDeviceGetAttribute(&p->num_sms, cudaDevAttrMultiProcessorCount, p->device);
   if (e != cudaSuccess) return cuda_fail("cudaDeviceGetAttribute", e);
-  e = cudaMalloc(reinterpret_cast<void**>(&p->flags), 256);
-  if (e != cudaSuccess) return cuda_fail("cudaMalloc(flags)", e);
-  e = cudaMemset(p->flags, 0, 256);
-  if (e != cudaSuccess) return cuda_fail("cudaMemset(flags)", e);
-  const size_t index = sizeof(int32_t) * (size_t)p->num_blocks * (p->block_size + 1);
-  e = cudaMalloc(reinterpret_cast<void**>(&p->slot_token), index);
+  // the status word, and the append index behind it
+  const size_t bytes = 256 + sizeof(int32_t) * (size_t)p->num_blocks * (p->block_size + 1);
+  e = cudaMalloc(reinterpret_cast<void**>(&p->flags), bytes);
   if (e != cudaSuccess) {
     cudaGetLastError();
-    set_last_error("cudaMalloc(append index, %zu): %s", index, cudaGetErrorString(e));
+    set_last_error("cudaMalloc(status word and append index, %zu): %s", bytes, cudaGetErrorString(e));
     return CLOVE_ERR_OOM;
   }
-  e = cudaMemset(p->slot_token, 0, index);
-  if (e != cudaSuccess) return cuda_fail("cudaMemset(append index)", e);
+  p->slot_token = p->flags + 64;
+  e = cudaMemset(p->flags, 0, bytes);
+  if (e != cudaSuccess) return cuda_fail("cudaMemset(status word and append index)", e);
   return fp8_encode_map(*p);
 }
 
@@ -188,7 +189,6 @@ int clove_fp8_pool_destroy(clove_fp8_pool_t pool) {
   OnDevice g(pool->device);
   if (pool->owns_memory) cudaFree(pool->codes);
   if (pool->flags) cudaFree(pool->flags);
-  if (pool->slot_token) cudaFree(pool->slot_token);
   delete pool;
   return CLOVE_OK;
 }

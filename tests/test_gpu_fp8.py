@@ -532,13 +532,15 @@ def test_c_refusals_and_created_pool():
     _lib.check(L.clove_fp8_pool_info(h, C.byref(info)))
     assert info.owns_memory == 1 and info.codes_bytes == 2 * 16 * 2 * 16 * 64 and info.mass and info.scales
     q = torch.ones((1, 4, 64), device=DEV)
-    bt, cl = i32([[0, 1]]), i32([20])
+    # a table wide enough for a call that needs scratch (a short one may not)
+    bt, cl = i32([[0, 1] + [0] * 126]), i32([20])
     out = torch.empty((1, 4, 64), device=DEV)
-    need = L.clove_fp8_decode_workspace_size(h, 1, 4, 32, 0)
+    need = L.clove_fp8_decode_workspace_size(h, 1, 4, 2048, 0)
+    assert need > 0
     ws = torch.empty(need + 256, dtype=torch.uint8, device=DEV)
 
     def decode(dtype=0, q=q.data_ptr(), k=None, v=None, out=out.data_ptr(), ws=ws.data_ptr(), n=need):
-        return L.clove_fp8_decode(h, dtype, q, k, v, 4, bt.data_ptr(), 2, cl.data_ptr(), 1, 0.1, 32, None, out, ws, n, None)
+        return L.clove_fp8_decode(h, dtype, q, k, v, 4, bt.data_ptr(), 128, cl.data_ptr(), 1, 0.1, 2048, None, out, ws, n, None)
 
     assert decode() == 0
     torch.cuda.synchronize()
