@@ -1391,6 +1391,12 @@ int launch_fp8_decode(const clove_fp8_pool& pool, const Fp8DecodeCall& c, cudaSt
     a.z_stride = L.z_stride;
   }
   a.direct = fp8_direct(pool, c.batch, c.scores.window > 0 ? std::min(c.scores.window, c.max_ctx) : c.max_ctx);
+  // the partition counts a CTA's share and 128 sequences' slices in 32 bits
+  const long long slices = (c.max_ctx + slice - 1LL) / slice + a.seg_cost;
+  if (slices > 0x7fffffffLL / 128 || slices * c.batch * pool.num_kv_heads / (2 * pool.num_sms) > 0x7fffffffLL) {
+    set_last_error("fp8_decode: batch %d of up to %d tokens is more than the partition counts", c.batch, c.max_ctx);
+    return CLOVE_ERR_UNSUPPORTED;
+  }
   a.append_here = a.append && (a.direct || slice == pool.block_size);
   switch (c.dtype) {
     case CLOVE_DTYPE_F32: return run_fp8_dim<float>(pool, a, stream);

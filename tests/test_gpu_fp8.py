@@ -250,6 +250,22 @@ def test_decode_lengths(lens, accumulate):
     run_decode(lens, 16, 2, 4, 128, torch.bfloat16, seed=sum(lens), accumulate=accumulate, poisoned=max(lens) < 5000)
 
 
+@pytest.mark.parametrize("H,G,append", [(4, 2, True), (5, 8, False)])
+def test_decode_large_batch(H, G, append):
+    # more sequences than a CTA has threads, empty ones among them
+    gen = torch.Generator().manual_seed(61)
+    lens = torch.randint(0, 90, (301,), generator=gen)
+    lens[::7], lens[128], lens[300] = 0, 1500, 700
+    run_decode(lens.tolist(), 16, H, G, 64, torch.bfloat16, seed=62, append=append, accumulate=append)
+
+
+@pytest.mark.parametrize("D,bs,dtype", [(128, 16, torch.bfloat16), (64, 256, torch.float32), (256, 64, torch.float16)])
+@pytest.mark.parametrize("n", [1000, 1024, 1025])
+def test_decode_whole_and_split_sequences(D, bs, dtype, n):
+    # short sequences are taken whole by a CTA, longer ones split: both sides of the border, with the last block shared
+    run_decode([n - 1, 3, 700], bs, 2, 4, D, dtype, seed=n + D, append=True)
+
+
 @pytest.mark.parametrize("max_extra", [1, 100, 5000])
 def test_decode_max_ctx_is_only_a_bound(max_extra):
     gen = torch.Generator().manual_seed(2)
@@ -374,6 +390,28 @@ def test_decode_is_reproducible():
         out = pool.decode(q, tables, i32(lens), max_ctx=max(lens), accumulate=True)
         runs.append((out.clone(), pool.mass.clone()))
     assert all(torch.equal(r[0], runs[0][0]) and torch.equal(r[1], runs[0][1]) for r in runs)
+
+
+@pytest.mark.parametrize("lens", [[600, 40], [5000, 900]], ids=["whole", "split"])
+def test_decode_stuck_wait_times_out_and_the_next_call_is_right(lens):
+    # the test hook leaves one stage unfilled: its reader's bounded wait runs
+    # out, the call ends and says so
+    gen = torch.Generator().manual_seed(56)
+    tables, nb = tables_for(lens, 16, gen)
+    pool = make_pool(nb, 16, 2, 128, gen)
+    ref = RefPool(pool.storage, pool.scales)
+    q = torch.randn((2, 8, 128), generator=gen)
+    L = _lib.lib()
+    try:
+        _lib.check(L.clove_cuda_debug_set(2000, 1))
+        pool.decode(q.to(DEV), tables, i32(lens), max_ctx=max(lens))
+        assert pool.pool_status() & _lib.FLAG_TIMEOUT
+    finally:
+        L.clove_cuda_debug_set(0, 0)
+    want, bound = ref.decode(q, tables, lens, 128 ** -0.5)
+    out = pool.decode(q.to(DEV), tables, i32(lens), max_ctx=max(lens))
+    assert pool.pool_status() == 0
+    assert ((out.cpu().double() - want).abs() <= bound).all()
 
 
 # ---------------------------------------------------------------------------
