@@ -501,11 +501,13 @@ __device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* map, const Smem
       for (int part = 0; part < 2; ++part) {
         const int s0 = part == 0 ? 0 : cut, s1 = part == 0 ? cut : nst;
         int s = s0;
-        if (first && a.inject_stall && s < s1) {  // test hook: the CTA's first stage is never filled
-          ++s;
-          ++slot;
+        if (first && s < s1) {
+          first = false;
+          if (a.inject_stall) {  // test hook: the CTA's first stage is never filled
+            ++s;
+            ++slot;
+          }
         }
-        first = false;
 #pragma unroll 1
         for (; s < s1; ++s) {
           if (slot == a.nstage) {
