@@ -1099,47 +1099,48 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
 // ---------------------------------------------------------------------------
 // weights: mass += sum over the group of 2^(z - M) / L
 // ---------------------------------------------------------------------------
-constexpr int kMassThreads = 256, kMassTokens = 128;  // tokens per warp and item: four per lane
+constexpr int kMassThreads = 256, kMassCtas = 8;  // CTAs per SM
+constexpr int kMassTokens = 128;                  // tokens per warp and step: four per lane
 
-// Items (sequence, KV head, 128 tokens), one warp each; those behind a
-// sequence's end cost a look at its length.
+// The warps are dealt out evenly to the (sequence, KV head) pairs, those of a
+// pair take its attended tokens 128 at a time.
 __global__ void __launch_bounds__(kMassThreads) fp8_mass_kernel(const Fp8Args a) {
   const int H = a.num_kv_heads, G = a.group, bs = a.real_block, lane = threadIdx.x & 31;
-  const int chunks = (a.max_ctx + kMassTokens - 1) / kMassTokens;
-  const long long total = (long long)a.batch * H * chunks;
+  const int heads = a.batch * H, warps = gridDim.x * (kMassThreads / 32), per = max(1, warps / heads);
+  const int id = blockIdx.x * (kMassThreads / 32) + (threadIdx.x >> 5);
   griddep_wait();
-  for (long long i = (long long)blockIdx.x * (kMassThreads / 32) + (threadIdx.x >> 5); i < total;
-       i += (long long)gridDim.x * (kMassThreads / 32)) {
-    const int head = (int)(i / chunks), b = head / H, h = head - b * H;
+  for (int head = id / per; head < heads; head += warps / per) {
+    const int b = head / H, h = head - b * H;
     const int L = clamp_ctx(a.context_lens, b, a.max_ctx, a.append);
     const int t0 = a.window > 0 ? max(0, L - a.window) : 0;
-    const int t = (int)(i - (long long)head * chunks) * kMassTokens + 4 * lane;  // this lane's first token
-    if (t >= L || t + 4 <= t0) continue;
-    int blk = __ldg(a.block_tables + (size_t)b * a.bt_stride + (t >> a.real_shift));
-    const bool bad = blk < 0 || blk >= a.num_blocks;
-    if (bad) blk = 0;
-    float* dst = a.mass + ((size_t)blk * H + h) * bs + (t & (bs - 1));
-    const float4 was = *reinterpret_cast<const float4*>(dst);
-    float w[4] = {0.f, 0.f, 0.f, 0.f};
-    const float* z = a.z + (size_t)head * G * a.z_stride + t;
+    for (int t = (t0 / kMassTokens + id % per) * kMassTokens + 4 * lane; t < L; t += per * kMassTokens) {
+      if (t + 4 <= t0) continue;
+      int blk = __ldg(a.block_tables + (size_t)b * a.bt_stride + (t >> a.real_shift));
+      const bool bad = blk < 0 || blk >= a.num_blocks;
+      if (bad) blk = 0;
+      float* dst = a.mass + ((size_t)blk * H + h) * bs + (t & (bs - 1));
+      const float4 was = *reinterpret_cast<const float4*>(dst);
+      float w[4] = {0.f, 0.f, 0.f, 0.f};
+      const float* z = a.z + (size_t)head * G * a.z_stride + t;
 #pragma unroll 4
-    for (int g = 0; g < G; ++g) {
-      const float2 st = __ldg(a.row_state + (size_t)head * G + g);
-      const float4 v = __ldcs(reinterpret_cast<const float4*>(z + (size_t)g * a.z_stride));
-      w[0] = fmaf(ex2(v.x - st.x), st.y, w[0]);
-      w[1] = fmaf(ex2(v.y - st.x), st.y, w[1]);
-      w[2] = fmaf(ex2(v.z - st.x), st.y, w[2]);
-      w[3] = fmaf(ex2(v.w - st.x), st.y, w[3]);
-    }
-    if (t >= t0 && t + 4 <= L - a.append) {
-      *reinterpret_cast<float4*>(dst) = make_float4(was.x + w[0], was.y + w[1], was.z + w[2], was.w + w[3]);
-    } else {
-      const float old[4] = {was.x, was.y, was.z, was.w};
+      for (int g = 0; g < G; ++g) {
+        const float2 st = __ldg(a.row_state + (size_t)head * G + g);
+        const float4 v = __ldcs(reinterpret_cast<const float4*>(z + (size_t)g * a.z_stride));
+        w[0] = fmaf(ex2(v.x - st.x), st.y, w[0]);
+        w[1] = fmaf(ex2(v.y - st.x), st.y, w[1]);
+        w[2] = fmaf(ex2(v.z - st.x), st.y, w[2]);
+        w[3] = fmaf(ex2(v.w - st.x), st.y, w[3]);
+      }
+      if (t >= t0 && t + 4 <= L - a.append) {
+        *reinterpret_cast<float4*>(dst) = make_float4(was.x + w[0], was.y + w[1], was.z + w[2], was.w + w[3]);
+      } else {
+        const float old[4] = {was.x, was.y, was.z, was.w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (t + k < t0 || t + k >= L) continue;
-        const bool mine = a.append && t + k == L - 1;  // the new token starts at its own weight
-        if (!(mine && bad)) dst[k] = mine ? w[k] : old[k] + w[k];
+        for (int k = 0; k < 4; ++k) {
+          if (t + k < t0 || t + k >= L) continue;
+          const bool mine = a.append && t + k == L - 1;  // the new token starts at its own weight
+          if (!(mine && bad)) dst[k] = mine ? w[k] : old[k] + w[k];
+        }
       }
     }
   }
@@ -1326,7 +1327,7 @@ static int run_fp8(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) 
   }
   if (a.z != nullptr) {
     const long long items = (long long)a.batch * a.num_kv_heads * ((a.max_ctx + kMassTokens - 1) / kMassTokens);
-    const dim3 grid((unsigned)std::min(items / (kMassThreads / 32) + 1, 8LL * pool.num_sms));
+    const dim3 grid((unsigned)std::min(items / (kMassThreads / 32) + 1, kMassCtas * (long long)pool.num_sms));
     rc = fp8_launch_status("fp8_decode weights launch", launch_chained(fp8_mass_kernel, grid, kMassThreads, 0, stream, a));
     if (rc) return rc;
     count_launches(1);

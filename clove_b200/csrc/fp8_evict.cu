@@ -96,6 +96,7 @@ __device__ __forceinline__ int2 peer_int2(uint32_t a) {
 template <int kSelThreads, int kPerSm>
 __global__ void __launch_bounds__(kSelThreads, kPerSm) fp8_select_kernel(const Fp8EvictArgs a, int C, int room) {
   constexpr int kSelWarps = kSelThreads / 32, kBinsPer = kBins / kSelThreads;
+  static_assert(kBinsPer % 4 == 0 && kBinsPer * kSelThreads == kBins, "a thread reads its bins four at a time");
   extern __shared__ uint32_t keys[];
   __shared__ __align__(16) int hist[kBins];
   __shared__ int warp_tot[kSelWarps];
