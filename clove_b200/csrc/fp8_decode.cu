@@ -1119,7 +1119,6 @@ __global__ void __launch_bounds__(kMassThreads) fp8_mass_kernel(const Fp8Args a)
       const bool bad = blk < 0 || blk >= a.num_blocks;
       if (bad) blk = 0;
       float* dst = a.mass + ((size_t)blk * H + h) * bs + (t & (bs - 1));
-      const float4 was = *reinterpret_cast<const float4*>(dst);
       float w[4] = {0.f, 0.f, 0.f, 0.f};
       const float* z = a.z + (size_t)head * G * a.z_stride + t;
 #pragma unroll 4
@@ -1131,15 +1130,18 @@ __global__ void __launch_bounds__(kMassThreads) fp8_mass_kernel(const Fp8Args a)
         w[2] = fmaf(ex2(v.z - st.x), st.y, w[2]);
         w[3] = fmaf(ex2(v.w - st.x), st.y, w[3]);
       }
+      // added atomically: forked sequences share blocks
       if (t >= t0 && t + 4 <= L - a.append) {
-        *reinterpret_cast<float4*>(dst) = make_float4(was.x + w[0], was.y + w[1], was.z + w[2], was.w + w[3]);
+        asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(dst), "f"(w[0]), "f"(w[1]), "f"(w[2]), "f"(w[3])
+                     : "memory");
       } else {
-        const float old[4] = {was.x, was.y, was.z, was.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if (t + k < t0 || t + k >= L) continue;
-          const bool mine = a.append && t + k == L - 1;  // the new token starts at its own weight
-          if (!(mine && bad)) dst[k] = mine ? w[k] : old[k] + w[k];
+          if (!a.append || t + k < L - 1)
+            atomicAdd(dst + k, w[k]);
+          else if (!bad)
+            dst[k] = w[k];  // the new token starts at its own weight
         }
       }
     }

@@ -66,7 +66,8 @@ typedef struct clove_fp8_pool_info {
  *   window > 0      only the last `window` tokens are attended to
  * accumulate != 0: the call adds each token's attention weight, summed over
  * the query heads of its KV head, to the pool's mass (a token the call
- * appends starts at its own weight). */
+ * appends starts at its own weight).  Sequences of one call may share blocks
+ * (forks): their weights add up, in an order that may change the last bit. */
 typedef struct clove_fp8_scores {
     float softcap;
     const float* alibi_slopes;

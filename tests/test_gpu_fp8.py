@@ -370,6 +370,30 @@ def test_decode_bad_tables_and_lengths_are_flagged():
     assert pool.pool_status() == 0
 
 
+@pytest.mark.parametrize("shared", [3, 80])
+def test_decode_forked_sequences_add_up_their_weights(shared):
+    # forks read the same blocks in one call; each appends to a block of its own
+    gen = torch.Generator().manual_seed(57)
+    bs, H, D, B = 16, 2, 64, 6
+    lens = [shared * bs + 5] * B
+    tables = torch.zeros((B, shared + 1), dtype=torch.int32)
+    tables[:, :shared] = torch.randperm(shared, generator=gen)
+    tables[:, shared] = shared + torch.arange(B)
+    tables = tables.to(DEV)
+    pool = make_pool(shared + B, bs, H, D, gen, mass=True, scales=(-10, -6))
+    ref = RefPool(pool.storage, pool.scales, pool.mass)
+    q = torch.randn((B, 8, D), generator=gen)
+    kv = torch.randn((2, B, H, D), generator=gen)
+    ref.append(kv[0], kv[1], (shared + torch.arange(B)) * bs + 5)
+    want, bound = ref.decode(q, tables, [n + 1 for n in lens], 0.125, accumulate=True)
+    out = pool.decode(q.to(DEV), tables, i32(lens), scale=0.125, max_ctx=lens[0] + 1, k_new=kv[0].to(DEV),
+                      v_new=kv[1].to(DEV), accumulate=True)
+    assert ((out.cpu().double() - want).abs() <= bound).all()
+    # B additions to one float32
+    assert ((pool.mass.cpu().double() - ref.mass).abs() <= ref.mass_bound + B * 2.0 ** -23 * ref.mass).all()
+    check_state(pool, ref)
+
+
 def test_decode_empty_batch_and_no_tokens():
     pool = make_pool(4, 16, 2, 64, torch.Generator().manual_seed(54))
     out = torch.full((2, 4, 64), 7.0, device=DEV)
