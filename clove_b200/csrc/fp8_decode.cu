@@ -30,8 +30,8 @@
 //     running maximum m), and multiplies weights by v_scale / vref <= 2;
 //   - the value sum of a pass (64 tokens; 32 for head_dim 256) starts from zero
 //     in the tensor cores and is added to f32 registers, so the chain of
-//     truncated tensor-core additions is four long, not as long as the
-//     sequence.
+//     truncated tensor-core additions is four long (eight where each half has
+//     its MMA), not as long as the sequence.
 //
 // Shared memory.  A tile is contiguous in HBM; it is copied as rows of 128
 // bytes (64 for head_dim 64) with the hardware swizzle: the 16-byte chunk at
@@ -1115,9 +1115,8 @@ __global__ void __launch_bounds__(kMassThreads) fp8_mass_kernel(const Fp8Args a)
     const int t0 = a.window > 0 ? max(0, L - a.window) : 0;
     for (int t = (t0 / kMassTokens + id % per) * kMassTokens + 4 * lane; t < L; t += per * kMassTokens) {
       if (t + 4 <= t0) continue;
-      int blk = __ldg(a.block_tables + (size_t)b * a.bt_stride + (t >> a.real_shift));
-      const bool bad = blk < 0 || blk >= a.num_blocks;
-      if (bad) blk = 0;
+      const int blk = __ldg(a.block_tables + (size_t)b * a.bt_stride + (t >> a.real_shift));
+      if (blk < 0 || blk >= a.num_blocks) continue;  // (flagged by the decode)
       float* dst = a.mass + ((size_t)blk * H + h) * bs + (t & (bs - 1));
       float w[4] = {0.f, 0.f, 0.f, 0.f};
       const float* z = a.z + (size_t)head * G * a.z_stride + t;
@@ -1140,7 +1139,7 @@ __global__ void __launch_bounds__(kMassThreads) fp8_mass_kernel(const Fp8Args a)
           if (t + k < t0 || t + k >= L) continue;
           if (!a.append || t + k < L - 1)
             atomicAdd(dst + k, w[k]);
-          else if (!bad)
+          else
             dst[k] = w[k];  // the new token starts at its own weight
         }
       }
@@ -1328,7 +1327,7 @@ static int run_fp8(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) 
     count_launches(1);
   }
   if (a.z != nullptr) {
-    const long long items = (long long)a.batch * a.num_kv_heads * ((a.max_ctx + kMassTokens - 1) / kMassTokens);
+    const long long items = (long long)a.batch * a.num_kv_heads * ((a.max_ctx + kMassTokens - 1LL) / kMassTokens);
     const dim3 grid((unsigned)std::min(items / (kMassThreads / 32) + 1, kMassCtas * (long long)pool.num_sms));
     rc = fp8_launch_status("fp8_decode weights launch", launch_chained(fp8_mass_kernel, grid, kMassThreads, 0, stream, a));
     if (rc) return rc;

@@ -370,6 +370,20 @@ def test_decode_bad_tables_and_lengths_are_flagged():
     assert pool.pool_status() == 0
 
 
+@pytest.mark.parametrize("append", [False, True])
+def test_decode_bad_tables_leave_other_weights_alone(append):
+    gen = torch.Generator().manual_seed(54)
+    pool = make_pool(8, 16, 2, 64, gen, mass=True)
+    pool.mass.zero_()
+    tables = torch.tensor([[3, 4, 5], [6, 99, -1]], dtype=torch.int32, device=DEV)
+    q = torch.randn((2, 4, 64), generator=gen).to(DEV)
+    kv = torch.randn((2, 2, 2, 64), generator=gen).to(DEV)
+    new = dict(k_new=kv[0], v_new=kv[1]) if append else {}
+    pool.decode(q, tables, i32([20, 40 - append]), max_ctx=40, accumulate=True, **new)
+    assert pool.pool_status() == _lib.FLAG_BLOCK_OOB
+    assert (pool.mass[[0, 1, 2, 7]] == 0).all() and (pool.mass[[3, 6]] > 0).all()
+
+
 @pytest.mark.parametrize("shared", [3, 80])
 def test_decode_forked_sequences_add_up_their_weights(shared):
     # forks read the same blocks in one call; each appends to a block of its own
