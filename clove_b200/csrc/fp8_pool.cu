@@ -1,5 +1,6 @@
 // The C ABI of the 8-bit cache (include/clove_fp8.h): argument checks, pool
 // lifecycle and error reporting around the kernel launchers.
+#include <exception>
 #include <new>
 
 #include "fp8_common.cuh"
@@ -85,6 +86,8 @@ int finish_pool(clove_fp8_pool* p) {
   }
   p->slot_token = p->flags + 64;
   e = cudaMemset(p->flags, 0, bytes);
+  // the first call may come on a stream that does not wait for this one
+  if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
   if (e != cudaSuccess) return cuda_fail("cudaMemset(status word and append index)", e);
   return fp8_encode_map(*p);
 }
@@ -323,7 +326,11 @@ int clove_fp8_decode(clove_fp8_pool_t pool, int dtype, const void* q, const void
   c.out = out;
   c.workspace = workspace;
   c.workspace_bytes = workspace_bytes;
-  return launch_fp8_decode(*pool, c, static_cast<cudaStream_t>(stream));
+  try {
+    return launch_fp8_decode(*pool, c, static_cast<cudaStream_t>(stream));
+  } catch (const std::exception&) {  // (the launch configurations' table)
+    return fail(CLOVE_ERR_OOM, "fp8_decode: out of host memory");
+  }
 }
 
 size_t clove_fp8_evict_workspace_size(clove_fp8_pool_t pool, int batch, int max_ctx, int budget) {

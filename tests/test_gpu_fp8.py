@@ -370,6 +370,32 @@ def test_decode_bad_tables_and_lengths_are_flagged():
     assert pool.pool_status() == 0
 
 
+def test_created_pool_is_clear_before_its_first_call():
+    """The codes' and the index's zeros are written before create returns, not
+    behind a call on a stream that does not wait for the creating one."""
+    lib, h = _lib.lib(), C.c_void_p()
+    nb, bs, H, D, n = 1 << 18, 16, 8, 64, 400
+    gen = torch.Generator().manual_seed(55)
+    kv = torch.randn((2, n, H, D), generator=gen).to(DEV)
+    slots = torch.arange(n, dtype=torch.int32, device=DEV)
+    table = torch.arange(n // bs, dtype=torch.int32, device=DEV)[None]
+    out = torch.empty((2, n, H, D), device=DEV)
+    ws = torch.empty(4 * n, dtype=torch.uint8, device=DEV)
+    lens, s = i32([n]), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    _lib.check(lib.clove_fp8_pool_create(0, nb, bs, H, D, 1, C.byref(h)))
+    try:
+        _lib.check(lib.clove_fp8_append(h, _lib.DTYPE_F32, kv[0].data_ptr(), kv[1].data_ptr(), slots.data_ptr(), n,
+                                        ws.data_ptr(), 4 * n, s.cuda_stream))
+        _lib.check(lib.clove_fp8_gather(h, table.data_ptr(), n // bs, lens.data_ptr(), 1, n, out[0].data_ptr(),
+                                        out[1].data_ptr(), s.cuda_stream))
+        s.synchronize()
+        # half a step of e4m3 (2^-4), or of its subnormals: 2^-10 of a scale <= 2 max / 448
+        assert ((out - kv).abs() <= kv.abs() * 2.0 ** -4 + kv.abs().max() * 2.0 ** -9 / 448).all()
+    finally:
+        lib.clove_fp8_pool_destroy(h)
+
+
 @pytest.mark.parametrize("append", [False, True])
 def test_decode_bad_tables_leave_other_weights_alone(append):
     gen = torch.Generator().manual_seed(54)
