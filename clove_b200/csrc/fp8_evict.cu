@@ -379,16 +379,21 @@ int launch_fp8_evict(const clove_fp8_pool& pool, const Fp8EvictCall& c, cudaStre
   a.num_blocks = pool.num_blocks;
   a.block_size = pool.block_size;
   a.num_kv_heads = pool.num_kv_heads;
-  // CTAs per (sequence, head): parts of at most 8192 tokens of the longest sequence (of 2048 while the GPU has room
-  // for more CTAs), in a cluster of up to 8.  Short parts alone on a CTA take few threads, so that many fit an SM.
   const int most = std::min(c.budget, c.max_ctx);
   const long long heads = (long long)c.batch * pool.num_kv_heads;
+  const int chunks = (int)((most + 31LL) / 32);
+  if (heads * chunks > 0x7fffffff - (1 << 20)) {
+    set_last_error("fp8_evict: %lld rows to move", heads * chunks * 32);
+    return CLOVE_ERR_UNSUPPORTED;
+  }
+  // CTAs per (sequence, head): parts of at most 8192 tokens of the longest sequence (of 2048 while the GPU has room
+  // for more CTAs), in a cluster of up to 8.  Short parts alone on a CTA take few threads, so that many fit an SM.
   int C = 1;
   while (C < 8 && (C * 8192LL < c.max_ctx || (C * 2048LL < c.max_ctx && 2 * C * heads <= 2 * pool.num_sms))) C *= 2;
   auto select = C == 1 ? fp8_select_kernel<256, 5> : fp8_select_kernel<512, 3>;
   const unsigned threads = C == 1 ? 256 : 512;
-  const int part = ((c.max_ctx + C - 1) / C + 511) / 512 * 512;
-  const int room = std::min(part, kMaxRoom), smem = room * (int)sizeof(uint32_t);
+  const long long part = ((c.max_ctx + C - 1LL) / C + 511) / 512 * 512;
+  const int room = (int)std::min<long long>(part, kMaxRoom), smem = room * (int)sizeof(uint32_t);
   int rc = fp8_launch_status("cudaFuncSetAttribute",
                              cudaFuncSetAttribute(select, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                   kMaxRoom * (int)sizeof(uint32_t)));
@@ -409,11 +414,6 @@ int launch_fp8_evict(const clove_fp8_pool& pool, const Fp8EvictCall& c, cudaStre
   if (rc) return rc;
   count_launches(1);
   if (most == 0) return CLOVE_OK;
-  const int chunks = (most + 31) / 32;
-  if (heads * chunks > 0x7fffffff - (1 << 20)) {
-    set_last_error("fp8_evict: %lld rows to move", heads * chunks * 32);
-    return CLOVE_ERR_UNSUPPORTED;
-  }
   cfg.gridDim = dim3((unsigned)std::min<long long>((heads * chunks + kCompactWarps - 1) / kCompactWarps,
                                                    (long long)pool.num_sms * kCompactPerSm));
   cfg.blockDim = dim3(kCompactWarps * 32);
