@@ -595,12 +595,42 @@ __device__ __forceinline__ void codes4(uint32_t w, uint32_t& lo, uint32_t& hi) {
       : "r"(w));
 }
 
-// x, y = hi + lo, each a pair of halves.
-__device__ __forceinline__ void split_halves(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
+// Two f32 operations in one instruction, each rounded as alone.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// v = hi + lo, each a pair of halves.
+__device__ __forceinline__ void split_halves(float2 v, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(v.x, v.y);
+  const float2 r = fma2(__half22float2(h), both(-1.f), v);
   hi = half2_bits(h);
-  lo = half2_bits(__floats2half2_rn(x - f.x, y - f.y));
+  lo = half2_bits(__floats2half2_rn(r.x, r.y));
 }
 
 // 16 bytes of elements, widened.
@@ -652,12 +682,16 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// tanh for |x| <= kTanhNear, where scores below a cap mostly are: the series
-// to x^9 (off by less than 2^-24 of the value there).
-constexpr float kTanhNear = 0.3f;
-__device__ __forceinline__ float tanh_near(float x) {
-  const float y = x * x;
-  return fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), x);
+// tanh for |x| <= kTanhNear, where scores below a cap mostly are: x + x^3 P(x^2)
+// with P of degree 3, fitted so that the largest relative error there is
+// smallest (1.6e-8, a quarter of 2^-24; Taylor's coefficients give that up to 0.3).
+constexpr float kTanhNear = 0.5f;
+__device__ __forceinline__ float2 tanh_near(float2 x) {
+  const float2 y = mul2(x, x);
+  float2 p = fma2(y, both(0.01724149f), both(-0.05304549f));
+  p = fma2(y, p, both(0.13325879f));
+  p = fma2(y, p, both(-0.33333144f));
+  return fma2(mul2(x, y), p, x);
 }
 __device__ __forceinline__ float rcp(float x) {
   float y;
@@ -745,7 +779,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
     // Query fragments: row g scaled by a power of two that puts its largest
     // element in [2^13, 2^14), undone in the score's factor.
     uint32_t qh[KJ * 4][2], ql[kTwoHalves ? KJ * 4 : 1][2];
-    float zf[2], slope[2];  // of queries 2 tq and 2 tq + 1: score = dot * K scale * zf, bias per token
+    float2 zf, slope;  // of queries 2 tq and 2 tq + 1: score = dot * K scale * zf, bias per token
     // stage gs belongs to warp gs % NCW (nstage is a multiple of NCW)
     const int j_first = ((cw - gbase) % NCW + NCW) % NCW;
     const bool mine = j_first < x.nstages;
@@ -771,19 +805,16 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
       if (e < -126) f *= 0.5f;
       f = kExtra && a.softcap > 0.f ? f / a.softcap : f * kLog2e;
       const float s = kExtra && a.slopes != nullptr && gq < group ? __ldg(a.slopes + x.h * group + gq) * kLog2e : 0.f;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        zf[c] = __shfl_sync(0xffffffffu, f, (2 * tq + c) * 4);
-        slope[c] = __shfl_sync(0xffffffffu, s, (2 * tq + c) * 4);
-      }
+      zf = make_float2(__shfl_sync(0xffffffffu, f, 8 * tq), __shfl_sync(0xffffffffu, f, 8 * tq + 4));
+      slope = make_float2(__shfl_sync(0xffffffffu, s, 8 * tq), __shfl_sync(0xffffffffu, s, 8 * tq + 4));
 #pragma unroll
       for (int j = 0; j < KJ; ++j)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const float* f4 = q + j * 16 + w * 4;
           uint32_t lo[2];
-          split_halves(f4[0] * up, f4[1] * up, qh[j * 4 + w][0], lo[0]);
-          split_halves(f4[2] * up, f4[3] * up, qh[j * 4 + w][1], lo[1]);
+          split_halves(make_float2(f4[0] * up, f4[1] * up), qh[j * 4 + w][0], lo[0]);
+          split_halves(make_float2(f4[2] * up, f4[3] * up), qh[j * 4 + w][1], lo[1]);
           if constexpr (kTwoHalves) {
             ql[j * 4 + w][0] = lo[0];
             ql[j * 4 + w][1] = lo[1];
@@ -796,11 +827,12 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
                       ? a.z + ((size_t)(x.b * a.num_kv_heads + x.h) * group + 2 * tq) * a.z_stride
                       : nullptr;
 
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, vref = 0.f;
-    // value sums: o[8 i + 2 k + c] is dim k (of 4) of half i of this lane's V units, query 2 tq + c
-    float o[D / 4];
+    float m[2] = {-INFINITY, -INFINITY}, vref = 0.f;
+    float2 l2 = make_float2(0.f, 0.f);
+    // value sums: o[4 i + k] is dim k (of 4) of half i of this lane's V units, queries 2 tq and 2 tq + 1
+    float2 o[D / 8];
 #pragma unroll
-    for (int n = 0; n < D / 4; ++n) o[n] = 0.f;
+    for (int n = 0; n < D / 8; ++n) o[n] = make_float2(0.f, 0.f);
 
     bool aborted = false;
     for (int j = j_first; j < x.nstages; j += NCW) {
@@ -828,7 +860,8 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
 #pragma unroll 1
       for (int p0 = 0; p0 < (TT == PT ? 1 : hi); p0 += PT) {
         // ---- scores: tile e is tokens p0 + 8 e + g, queries 2 tq + c ----
-        float z[NE][2], wv[NE];
+        float2 z[NE];
+        float wv[NE];
         float vmax = 0.f;
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
@@ -860,33 +893,26 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
             const uint2 f = lds64(sbase + ((s_first + ((p0 + 8 * e) >> vshift)) & (kSclRing - 1)) * 8);
             wv[e] = __uint_as_float(f.y);
             vmax = fmaxf(vmax, wv[e]);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) z[e][c] = s[2 * r + c] * (__uint_as_float(f.x) * zf[c]);
+            z[e] = mul2(make_float2(s[2 * r], s[2 * r + 1]), mul2(both(__uint_as_float(f.x)), zf));
           }
         }
         if constexpr (kExtra) {
           if (cap > 0.f) {
             float most = 0.f;
 #pragma unroll
-            for (int e = 0; e < NE; ++e) most = fmaxf(most, fmaxf(fabsf(z[e][0]), fabsf(z[e][1])));
+            for (int e = 0; e < NE; ++e) most = fmaxf(most, fmaxf(fabsf(z[e].x), fabsf(z[e].y)));
             if (__any_sync(0xffffffffu, most > kTanhNear)) {
 #pragma unroll
-              for (int e = 0; e < NE; ++e)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) z[e][c] = tanh_any(z[e][c]) * cap;
+              for (int e = 0; e < NE; ++e) z[e] = make_float2(tanh_any(z[e].x) * cap, tanh_any(z[e].y) * cap);
             } else {
 #pragma unroll
-              for (int e = 0; e < NE; ++e)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) z[e][c] = tanh_near(z[e][c]) * cap;
+              for (int e = 0; e < NE; ++e) z[e] = mul2(tanh_near(z[e]), both(cap));
             }
           }
           if (a.slopes != nullptr) {
             const float back = (float)(t_base + p0 + g - (x.L - 1));  // exact below 2^24
 #pragma unroll
-            for (int e = 0; e < NE; ++e)
-#pragma unroll
-              for (int c = 0; c < 2; ++c) z[e][c] = fmaf(slope[c], back + (float)(8 * e), z[e][c]);
+            for (int e = 0; e < NE; ++e) z[e] = fma2(slope, both(back + (float)(8 * e)), z[e]);
           }
           if (zrow != nullptr) {
             const int left = hi - p0 - g;  // tokens of this lane's column
@@ -896,7 +922,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
               if (2 * tq + c < group) {
 #pragma unroll
                 for (int e = 0; e < NE; ++e)
-                  if (8 * e < left) zt[8 * e] = z[e][c];
+                  if (8 * e < left) zt[8 * e] = c ? z[e].y : z[e].x;
               }
               zt += a.z_stride;
             }
@@ -906,7 +932,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
 #pragma unroll
           for (int e = 0; e < NE; ++e) {
             const int tok = p0 + 8 * e + g;
-            if (tok < lo || tok >= hi) z[e][0] = z[e][1] = -INFINITY;
+            if (tok < lo || tok >= hi) z[e] = both(-INFINITY);
           }
         }
         // ---- online softmax of queries 2 tq and 2 tq + 1 ----
@@ -914,31 +940,30 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
         float corr[2], ms[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float mx = z[0][c];
+          float mx = c ? z[0].y : z[0].x;
 #pragma unroll
-          for (int e = 1; e < NE; ++e) mx = fmaxf(mx, z[e][c]);
+          for (int e = 1; e < NE; ++e) mx = fmaxf(mx, c ? z[e].y : z[e].x);
 #pragma unroll
           for (int s = 4; s < 32; s <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
           const float mn = fmaxf(m[c], mx);
-          ms[c] = mn == -INFINITY ? 0.f : mn - 14.f;
+          ms[c] = mn == -INFINITY ? 0.f : 14.f - mn;
           corr[c] = m[c] == -INFINITY ? 0.f : ex2(m[c] - mn);
           m[c] = mn;
-          l[c] *= corr[c];
         }
+        l2 = mul2(l2, make_float2(corr[0], corr[1]));
         // the P^T operand (tokens x queries): both halves of the weights, or, where columns 4..7 repeat the queries,
         // the high halves in columns 0..3 and the low ones in 4..7
         uint32_t ph[NE], pl[kTwin ? 1 : NE];
 #pragma unroll
         for (int e = 0; e < NE; ++e) {
-          const float p0e = ex2(z[e][0] - ms[0]), p1e = ex2(z[e][1] - ms[1]), f = wv[e] * vinv;
-          l[0] += p0e;
-          l[1] += p1e;
+          const float2 d = add2(z[e], make_float2(ms[0], ms[1])), w = make_float2(ex2(d.x), ex2(d.y));
+          l2 = add2(l2, w);
           uint32_t hi2, lo2;
-          split_halves(p0e * f, p1e * f, hi2, lo2);
+          split_halves(mul2(w, both(wv[e] * vinv)), hi2, lo2);
           ph[e] = transpose8x8(kTwin && tq >= 2 ? lo2 : hi2);
           if constexpr (!kTwin) pl[e] = transpose8x8(lo2);
         }
-        const float oc[2] = {corr[0] * (vref * vinv), corr[1] * (vref * vinv)};
+        const float2 oc = mul2(make_float2(corr[0], corr[1]), both(vref * vinv));
         vref = vnew;
         // ---- value sum, V^T (16 dims) times P^T (8 queries) ----
 #pragma unroll
@@ -977,9 +1002,9 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                float& on = o[(u * 2 + w) * 8 + 4 * i + r];
-                on = fmaf(on, oc[r & 1], d[i][r]);
+              for (int r = 0; r < 2; ++r) {
+                float2& on = o[(u * 2 + w) * 4 + 2 * i + r];
+                on = fma2(on, oc, make_float2(d[i][2 * r], d[i][2 * r + 1]));
               }
           }
         }
@@ -994,16 +1019,19 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
     // ---- hand-off: the last warp to finish a piece merges the others' states
     // (acc, m - 14, l), left in scratch, with its own, still in registers.
     // Lane (g, tq) holds queries 2 tq and 2 tq + 1 of its V units' dims. ----
+    float l[2] = {l2.x, l2.y};
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int s = 4; s < 32; s <<= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], s);
     if constexpr (kTwin) {  // high and low halves' sums
 #pragma unroll
-      for (int n = 0; n < D / 4; ++n) o[n] += __shfl_xor_sync(0xffffffffu, o[n], 2);
+      for (int n = 0; n < D / 8; ++n)
+        o[n] = add2(o[n], make_float2(__shfl_xor_sync(0xffffffffu, o[n].x, 2), __shfl_xor_sync(0xffffffffu, o[n].y, 2)));
     }
 #pragma unroll
-    for (int n = 0; n < D / 4; ++n) o[n] *= vref;
+    for (int n = 0; n < D / 8; ++n) o[n] = mul2(o[n], both(vref));
+    auto sum = [&](int n, int c) { return c ? o[n].y : o[n].x; };
     const uint32_t par = (uint32_t)n_done & 1u;
     if (!wait_or_abort(a, sm, &sm.scr_empty[0], par ^ 1u)) return;
     int order = 0;
@@ -1021,7 +1049,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
 #pragma unroll
           for (int i = 0; i < VH * VP * 2; ++i)
             *reinterpret_cast<float4*>(row + (i / (2 * VP)) * 128 + v_unit<D>(g, (i >> 1) % VP) * 8 + (i & 1) * 4) =
-                make_float4(o[8 * i + c], o[8 * i + 2 + c], o[8 * i + 4 + c], o[8 * i + 6 + c]);
+                make_float4(sum(4 * i, c), sum(4 * i + 1, c), sum(4 * i + 2, c), sum(4 * i + 3, c));
         }
         if (g == 0) {
           row[D] = m[c] - 14.f;
@@ -1068,10 +1096,10 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
           float4 va = make_float4(0.f, 0.f, 0.f, 0.f), vb = va;
           if (fa > 0.f) va = *reinterpret_cast<const float4*>(A + d);
           if (fb > 0.f) vb = *reinterpret_cast<const float4*>(B + d);
-          *reinterpret_cast<float4*>(dst + d) = make_float4(add(fo, o[8 * i + c], fa, va.x, fb, vb.x) * norm,
-                                                            add(fo, o[8 * i + 2 + c], fa, va.y, fb, vb.y) * norm,
-                                                            add(fo, o[8 * i + 4 + c], fa, va.z, fb, vb.z) * norm,
-                                                            add(fo, o[8 * i + 6 + c], fa, va.w, fb, vb.w) * norm);
+          *reinterpret_cast<float4*>(dst + d) = make_float4(add(fo, sum(4 * i, c), fa, va.x, fb, vb.x) * norm,
+                                                            add(fo, sum(4 * i + 1, c), fa, va.y, fb, vb.y) * norm,
+                                                            add(fo, sum(4 * i + 2, c), fa, va.z, fb, vb.z) * norm,
+                                                            add(fo, sum(4 * i + 3, c), fa, va.w, fb, vb.w) * norm);
         }
         if (g == 0) {
           if (!x.complete) {
