@@ -901,9 +901,15 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
             float most = 0.f;
 #pragma unroll
             for (int e = 0; e < NE; ++e) most = fmaxf(most, fmaxf(fabsf(z[e].x), fabsf(z[e].y)));
-            if (__any_sync(0xffffffffu, most > kTanhNear)) {
+            if (__builtin_expect(__any_sync(0xffffffffu, most > kTanhNear), 0)) {
+              // a loop of one body, the registers moving through it: unrolled it would crowd the instruction cache
+#pragma unroll 1
+              for (int i = 0; i < NE; ++i) {
+                const float2 w = make_float2(tanh_any(z[0].x) * cap, tanh_any(z[0].y) * cap);
 #pragma unroll
-              for (int e = 0; e < NE; ++e) z[e] = make_float2(tanh_any(z[e].x) * cap, tanh_any(z[e].y) * cap);
+                for (int e = 0; e < NE - 1; ++e) z[e] = z[e + 1];
+                z[NE - 1] = w;
+              }
             } else {
 #pragma unroll
               for (int e = 0; e < NE; ++e) z[e] = mul2(tanh_near(z[e]), both(cap));
