@@ -719,10 +719,11 @@ __device__ __forceinline__ float floor_pow2(float x) {
 }
 __device__ __forceinline__ float inv_pow2(float x) { return __int_as_float((254 << 23) - __float_as_int(x)); }
 
-// kExtra: scores may be capped, biased or kept; kTwin: groups of up to 4
-// queries.  (A variant has none of the others' code: what a pass runs has to
-// fit the instruction cache.)
-template <typename T, int D, int NCW, bool kExtra, bool kTwin>
+// kShaped: scores may be capped or biased; kKept: they are written out for the
+// weights; kTwin: groups of up to 4 queries.  A variant has none of the others'
+// code, run or not: it would crowd the instruction cache (the capped window of
+// 256 sequences took 121 us with the code that keeps scores beside it, 111 without).
+template <typename T, int D, int NCW, bool kShaped, bool kKept, bool kTwin>
 __global__ void __launch_bounds__((NCW + 1) * 32, 2)
     fp8_decode_kernel(const __grid_constant__ CUtensorMap map, const Fp8Args a) {
   static_assert(NCW == 3, "the hand-off sums three warps' states");
@@ -803,8 +804,8 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
       const float up = __int_as_float((127 - max(e, -127)) << 23);
       float f = a.scale * __int_as_float((127 + max(e, -126)) << 23);
       if (e < -126) f *= 0.5f;
-      f = kExtra && a.softcap > 0.f ? f / a.softcap : f * kLog2e;
-      const float s = kExtra && a.slopes != nullptr && gq < group ? __ldg(a.slopes + x.h * group + gq) * kLog2e : 0.f;
+      f = kShaped && a.softcap > 0.f ? f / a.softcap : f * kLog2e;
+      const float s = kShaped && a.slopes != nullptr && gq < group ? __ldg(a.slopes + x.h * group + gq) * kLog2e : 0.f;
       zf = make_float2(__shfl_sync(0xffffffffu, f, 8 * tq), __shfl_sync(0xffffffffu, f, 8 * tq + 4));
       slope = make_float2(__shfl_sync(0xffffffffu, s, 8 * tq), __shfl_sync(0xffffffffu, s, 8 * tq + 4));
 #pragma unroll
@@ -823,9 +824,8 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
     }
     const float cap = a.softcap * kLog2e;
     const int t_first = a.window > 0 ? max(0, x.L - a.window) : 0;  // first token attended to
-    float* zrow = kExtra && a.z != nullptr
-                      ? a.z + ((size_t)(x.b * a.num_kv_heads + x.h) * group + 2 * tq) * a.z_stride
-                      : nullptr;
+    float* zrow =
+        kKept ? a.z + ((size_t)(x.b * a.num_kv_heads + x.h) * group + 2 * tq) * a.z_stride : nullptr;
 
     float m[2] = {-INFINITY, -INFINITY}, vref = 0.f;
     float2 l2 = make_float2(0.f, 0.f);
@@ -896,7 +896,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
             z[e] = mul2(make_float2(s[2 * r], s[2 * r + 1]), mul2(both(__uint_as_float(f.x)), zf));
           }
         }
-        if constexpr (kExtra) {
+        if constexpr (kShaped) {
           if (cap > 0.f) {
             float most = 0.f;
 #pragma unroll
@@ -920,18 +920,18 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
 #pragma unroll
             for (int e = 0; e < NE; ++e) z[e] = fma2(slope, both(back + (float)(8 * e)), z[e]);
           }
-          if (zrow != nullptr) {
-            const int left = hi - p0 - g;  // tokens of this lane's column
-            float* zt = zrow + t_base + p0 + g;
+        }
+        if constexpr (kKept) {
+          const int left = hi - p0 - g;  // tokens of this lane's column
+          float* zt = zrow + t_base + p0 + g;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              if (2 * tq + c < group) {
+          for (int c = 0; c < 2; ++c) {
+            if (2 * tq + c < group) {
 #pragma unroll
-                for (int e = 0; e < NE; ++e)
-                  if (8 * e < left) zt[8 * e] = c ? z[e].y : z[e].x;
-              }
-              zt += a.z_stride;
+              for (int e = 0; e < NE; ++e)
+                if (8 * e < left) zt[8 * e] = c ? z[e].y : z[e].x;
             }
+            zt += a.z_stride;
           }
         }
         if (ragged) {
@@ -1111,7 +1111,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
           if (!x.complete) {
             dst[D] = M;
             dst[D + 1] = L;
-          } else if (kExtra && a.row_state != nullptr) {
+          } else if (kKept) {
             a.row_state[(size_t)x.b * Hq + hq] = make_float2(M, inv);
           }
         }
@@ -1283,12 +1283,12 @@ struct Fp8Cfg {
   int nstage, smem, ctas;
 };
 
-template <typename T, int D, bool kExtra, bool kTwin>
+template <typename T, int D, bool kShaped, bool kKept, bool kTwin>
 static int fp8_cfg(const clove_fp8_pool& pool, int slice, int group, Fp8Cfg* out) {
   static std::mutex mu;
   static std::unordered_map<long long, Fp8Cfg> cache;
   static std::unordered_map<int, int> attr;  // device -> shared memory the kernel may use there
-  auto kern = fp8_decode_kernel<T, D, kFp8Warps, kExtra, kTwin>;
+  auto kern = fp8_decode_kernel<T, D, kFp8Warps, kShaped, kKept, kTwin>;
   const long long key = ((long long)pool.device << 32) | ((long long)slice << 8) | group;
   std::lock_guard<std::mutex> lk(mu);
   auto it = cache.find(key);
@@ -1329,11 +1329,11 @@ static int fp8_cfg(const clove_fp8_pool& pool, int slice, int group, Fp8Cfg* out
   return CLOVE_OK;
 }
 
-template <typename T, int D, bool kExtra, bool kTwin>
+template <typename T, int D, bool kShaped, bool kKept, bool kTwin>
 static int run_fp8(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) {
   a.stage_blocks = stage_tokens(D) / a.block_size;
   Fp8Cfg c;
-  int rc = fp8_cfg<T, D, kExtra, kTwin>(pool, a.block_size, a.group, &c);
+  int rc = fp8_cfg<T, D, kShaped, kKept, kTwin>(pool, a.block_size, a.group, &c);
   if (rc) return rc;
   a.nstage = c.nstage;
   a.ncw = kFp8Warps;
@@ -1349,7 +1349,7 @@ static int run_fp8(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) 
     count_launches(1);
   }
   rc = fp8_launch_status("fp8_decode launch",
-                         launch_chained(fp8_decode_kernel<T, D, kFp8Warps, kExtra, kTwin>, dim3(a.num_ctas), (kFp8Warps + 1) * 32,
+                         launch_chained(fp8_decode_kernel<T, D, kFp8Warps, kShaped, kKept, kTwin>, dim3(a.num_ctas), (kFp8Warps + 1) * 32,
                                         c.smem, stream, pool.map, a));
   if (rc) return rc;
   count_launches(1);
@@ -1372,9 +1372,15 @@ static int run_fp8(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) 
 
 template <typename T, int D>
 static int run_fp8_scores(const clove_fp8_pool& pool, Fp8Args& a, cudaStream_t stream) {
-  const bool extra = a.softcap > 0.f || a.slopes != nullptr || a.z != nullptr;
-  if (a.group <= 4) return extra ? run_fp8<T, D, true, true>(pool, a, stream) : run_fp8<T, D, false, true>(pool, a, stream);
-  return extra ? run_fp8<T, D, true, false>(pool, a, stream) : run_fp8<T, D, false, false>(pool, a, stream);
+  auto run = [&](auto twin) {
+    const bool shaped = a.softcap > 0.f || a.slopes != nullptr;
+    if (a.z != nullptr)
+      return shaped ? run_fp8<T, D, true, true, twin.value>(pool, a, stream)
+                    : run_fp8<T, D, false, true, twin.value>(pool, a, stream);
+    return shaped ? run_fp8<T, D, true, false, twin.value>(pool, a, stream)
+                  : run_fp8<T, D, false, false, twin.value>(pool, a, stream);
+  };
+  return a.group <= 4 ? run(std::true_type{}) : run(std::false_type{});
 }
 
 template <typename T>
