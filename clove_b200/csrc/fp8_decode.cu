@@ -1136,46 +1136,112 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
 constexpr int kMassThreads = 256, kMassCtas = 8;  // CTAs per SM
 constexpr int kMassTokens = 128;                  // tokens per warp and step: four per lane
 
-// The warps are dealt out evenly to the (sequence, KV head) pairs, those of a
-// pair take its attended tokens 128 at a time.
+// The steps of all (sequence, KV head) pairs are one stream, sequence by
+// sequence, and every warp takes an equal run of it: with lengths that differ
+// the longest sequence would otherwise hold its warps several times as long as
+// the others theirs.
 __global__ void __launch_bounds__(kMassThreads) fp8_mass_kernel(const Fp8Args a) {
-  const int H = a.num_kv_heads, G = a.group, bs = a.real_block, lane = threadIdx.x & 31;
-  const int heads = a.batch * H, warps = gridDim.x * (kMassThreads / 32), per = max(1, warps / heads);
-  const int id = blockIdx.x * (kMassThreads / 32) + (threadIdx.x >> 5);
+  constexpr int kWarps = kMassThreads / 32;
+  __shared__ int warp_tot[kWarps], start[kMassThreads], count[kMassThreads];
+  __shared__ long long s_rest;
+  const int H = a.num_kv_heads, G = a.group, bs = a.real_block, tid = threadIdx.x, lane = tid & 31;
   griddep_wait();
-  for (int head = id / per; head < heads; head += warps / per) {
-    const int b = head / H, h = head - b * H;
+  // steps of one KV head of sequence b: from the first attended token's to the last's
+  auto first_step = [&](int L) { return a.window > 0 ? max(0, L - a.window) / kMassTokens : 0; };
+  auto steps = [&](int b) {
+    if (b >= a.batch) return 0;
     const int L = clamp_ctx(a.context_lens, b, a.max_ctx, a.append);
-    const int t0 = a.window > 0 ? max(0, L - a.window) : 0;
-    for (int t = (t0 / kMassTokens + id % per) * kMassTokens + 4 * lane; t < L; t += per * kMassTokens) {
-      if (t + 4 <= t0) continue;
-      const int blk = __ldg(a.block_tables + (size_t)b * a.bt_stride + (t >> a.real_shift));
-      if (blk < 0 || blk >= a.num_blocks) continue;  // (flagged by the decode)
-      float* dst = a.mass + ((size_t)blk * H + h) * bs + (t & (bs - 1));
-      float w[4] = {0.f, 0.f, 0.f, 0.f};
-      const float* z = a.z + (size_t)head * G * a.z_stride + t;
-#pragma unroll 4
-      for (int g = 0; g < G; ++g) {
-        const float2 st = __ldg(a.row_state + (size_t)head * G + g);
-        const float4 v = __ldcs(reinterpret_cast<const float4*>(z + (size_t)g * a.z_stride));
-        w[0] = fmaf(ex2(v.x - st.x), st.y, w[0]);
-        w[1] = fmaf(ex2(v.y - st.x), st.y, w[1]);
-        w[2] = fmaf(ex2(v.z - st.x), st.y, w[2]);
-        w[3] = fmaf(ex2(v.w - st.x), st.y, w[3]);
+    return (L + kMassTokens - 1) / kMassTokens - first_step(L);
+  };
+  int n = steps(tid), tot;
+  int before = block_excl_scan(n, warp_tot, &tot);
+  long long all = tot;
+  if (a.batch > kMassThreads) {
+    if (tid == 0) s_rest = 0;
+    __syncthreads();
+    long long mine = 0;
+#pragma unroll 1
+    for (int b = tid + kMassThreads; b < a.batch; b += kMassThreads) mine += steps(b);
+    if (mine) atomicAdd(reinterpret_cast<unsigned long long*>(&s_rest), (unsigned long long)mine);
+    __syncthreads();
+    all += s_rest;
+  }
+  all *= H;
+  const long long runs = (long long)gridDim.x * kWarps, run = (long long)blockIdx.x * kWarps + (tid >> 5);
+  const long long per = (all + runs - 1) / runs, lo = min(all, run * per);
+  const long long lo_last = min(all, ((long long)blockIdx.x * kWarps + kWarps - 1) * per);  // the CTA's last warp's
+  int left = (int)(min(all, lo + per) - lo);
+  // where the run starts
+  int b = -1, h = 0, c = 0, len = 0;
+  long long carry = 0;
+#pragma unroll 1
+  for (int base = 0;; ) {
+    start[tid] = before;
+    count[tid] = n;
+    __syncthreads();
+    if (left > 0 && b < 0 && lo < (carry + tot) * H) {
+#pragma unroll 1
+      for (int k = 0; b < 0 && k < kWarps; ++k) {
+        const long long s0 = (carry + start[32 * k + lane]) * H;
+        const unsigned hit = __ballot_sync(0xffffffffu, s0 <= lo && lo < s0 + (long long)count[32 * k + lane] * H);
+        if (hit == 0) continue;
+        const int at = 32 * k + __ffs(hit) - 1, r = (int)(lo - (carry + start[at]) * H);
+        b = base + at;
+        len = count[at];
+        h = r / len;
+        c = r - h * len;
       }
-      // added atomically: forked sequences share blocks
-      if (t >= t0 && t + 4 <= L - a.append) {
-        asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(dst), "f"(w[0]), "f"(w[1]), "f"(w[2]), "f"(w[3])
-                     : "memory");
-      } else {
+    }
+    carry += tot;
+    base += kMassThreads;
+    if (base >= a.batch || lo_last < carry * H) break;
+    __syncthreads();
+    n = steps(base + tid);
+    before = block_excl_scan(n, warp_tot, &tot);
+  }
+  if (b < 0) return;
+  int L = clamp_ctx(a.context_lens, b, a.max_ctx, a.append);
+  for (; left > 0; --left, ++c) {
+    if (c == len) {  // the next KV head, or the next sequence that has tokens
+      c = 0;
+      if (++h == H) {
+        h = 0;
+        do {
+          if (++b >= a.batch) return;  // (cannot happen while steps are left)
+          len = steps(b);
+        } while (len == 0);
+        L = clamp_ctx(a.context_lens, b, a.max_ctx, a.append);
+      }
+    }
+    const int head = b * H + h, t0 = a.window > 0 ? max(0, L - a.window) : 0;
+    const int t = (first_step(L) + c) * kMassTokens + 4 * lane;
+    if (t >= L || t + 4 <= t0) continue;
+    const int blk = __ldg(a.block_tables + (size_t)b * a.bt_stride + (t >> a.real_shift));
+    if (blk < 0 || blk >= a.num_blocks) continue;  // (flagged by the decode)
+    float* dst = a.mass + ((size_t)blk * H + h) * bs + (t & (bs - 1));
+    float w[4] = {0.f, 0.f, 0.f, 0.f};
+    const float* z = a.z + (size_t)head * G * a.z_stride + t;
+#pragma unroll 4
+    for (int g = 0; g < G; ++g) {
+      const float2 st = __ldg(a.row_state + (size_t)head * G + g);
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(z + (size_t)g * a.z_stride));
+      w[0] = fmaf(ex2(v.x - st.x), st.y, w[0]);
+      w[1] = fmaf(ex2(v.y - st.x), st.y, w[1]);
+      w[2] = fmaf(ex2(v.z - st.x), st.y, w[2]);
+      w[3] = fmaf(ex2(v.w - st.x), st.y, w[3]);
+    }
+    // added atomically: forked sequences share blocks
+    if (t >= t0 && t + 4 <= L - a.append) {
+      asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(dst), "f"(w[0]), "f"(w[1]), "f"(w[2]), "f"(w[3])
+                   : "memory");
+    } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (t + k < t0 || t + k >= L) continue;
-          if (!a.append || t + k < L - 1)
-            atomicAdd(dst + k, w[k]);
-          else
-            dst[k] = w[k];  // the new token starts at its own weight
-        }
+      for (int k = 0; k < 4; ++k) {
+        if (t + k < t0 || t + k >= L) continue;
+        if (!a.append || t + k < L - 1)
+          atomicAdd(dst + k, w[k]);
+        else
+          dst[k] = w[k];  // the new token starts at its own weight
       }
     }
   }
