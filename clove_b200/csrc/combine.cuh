@@ -137,6 +137,8 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const Args a) 
   __shared__ float rowv[24];
   __shared__ int pieces[kCombineMaxPieces];
   __shared__ int s_np;
+  // the kernel behind may set itself up now (it waits for this one before it reads results)
+  if constexpr (Args::kKeepsRowState) griddep_launch_dependents();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if constexpr (kTrace) {
     if (a.trace && threadIdx.x == 0) atomicMin(a.trace + 2, gtime());

@@ -1145,7 +1145,6 @@ __global__ void __launch_bounds__(kMassThreads) fp8_mass_kernel(const Fp8Args a)
   __shared__ int warp_tot[kWarps], start[kMassThreads], count[kMassThreads];
   __shared__ long long s_rest;
   const int H = a.num_kv_heads, G = a.group, bs = a.real_block, tid = threadIdx.x, lane = tid & 31;
-  griddep_wait();
   // steps of one KV head of sequence b: from the first attended token's to the last's
   auto first_step = [&](int L) { return a.window > 0 ? max(0, L - a.window) / kMassTokens : 0; };
   auto steps = [&](int b) {
@@ -1199,6 +1198,7 @@ __global__ void __launch_bounds__(kMassThreads) fp8_mass_kernel(const Fp8Args a)
     n = steps(base + tid);
     before = block_excl_scan(n, warp_tot, &tot);
   }
+  griddep_wait();  // (the lengths were complete before the decode let this kernel be launched)
   if (b < 0) return;
   int L = clamp_ctx(a.context_lens, b, a.max_ctx, a.append);
   for (; left > 0; --left, ++c) {
