@@ -6,7 +6,9 @@
 // that the call writes to it, finds their largest magnitude, settles the
 // scale, and stores the codes (rounding the rows already there when the scale
 // grows).  HBM bounds it for prompts (3 bytes per element with 16-bit input:
-// read 2, write 1), launch latency for a decode step.
+// read 2, write 1), launch latency for a decode step.  Measured with 8 heads of
+// 128, bf16: 8 x 2048 tokens 30 us (3.4 TB/s; ~4 us of it the first kernel),
+// 64 x 2048 5.0 TB/s, one token of each of 128 sequences 4 us.
 #include <algorithm>
 #include <type_traits>
 

@@ -259,6 +259,14 @@ def test_decode_large_batch(H, G, append):
     run_decode(lens.tolist(), 16, H, G, 64, torch.bfloat16, seed=62, append=append, accumulate=append)
 
 
+@pytest.mark.parametrize("softcap", [0.5, 3.0, 10.0, 40.0, 200.0])
+@pytest.mark.parametrize("G,D,accumulate", [(4, 128, False), (8, 64, True), (2, 256, True), (1, 128, False)])
+def test_decode_cap_from_flat_to_steep(softcap, G, D, accumulate):
+    # scores far below the cap, around it and far beyond it: all ranges of the tanh, alone and mixed
+    run_decode([300, 1, 70, 1500], 16, 2, G, D, torch.float16, seed=int(10 * softcap) + G, append=True, softcap=softcap,
+               alibi=G == 4, accumulate=accumulate)
+
+
 @pytest.mark.parametrize("D,bs,dtype", [(128, 16, torch.bfloat16), (64, 256, torch.float32), (256, 64, torch.float16)])
 @pytest.mark.parametrize("n", [1000, 1024, 1025])
 def test_decode_whole_and_split_sequences(D, bs, dtype, n):
