@@ -22,18 +22,28 @@
 //     row is scaled to the top of the f16 range (bf16 elements 2^-31 below the
 //     row's largest lose bits), an f32 query the sum of two halves and so two
 //     MMAs;
-//   - a weight is the sum of two halves, and the value sum is transposed too:
-//     V^T (16 dims) times P^T (8 queries).  With up to 4 queries columns 4..7
-//     repeat queries 0..3, and one MMA takes the high halves in columns 0..3
-//     and the low halves in 4..7 (their sums meet once a piece); with more,
-//     each half has its MMA.  An 8x8 transpose of f16 pairs (movmatrix) turns
-//     the score fragment into that operand;
-//   - weights are 2^(z - m + 14): the f16 range below the largest weight is 14
-//     binades longer than with 2^(z - m), so a weight is off by at most 2^-39
-//     of the row's largest however many light tokens there are;
-//   - the scales of V differ from block to block: a warp keeps the largest
-//     power of two seen, `vref`, in its accumulators' unit (as it keeps the
-//     running maximum m), and multiplies weights by v_scale / vref <= 2;
+//   - a weight times its block's V scale is the sum of two halves, off by at
+//     most 2^-23 of itself, and the value sum is transposed too: V^T (16 dims)
+//     times P^T (8 queries).  With up to 4 queries columns 4..7 repeat queries
+//     0..3, and one MMA takes the high halves in columns 0..3 and the low
+//     halves in 4..7 (their sums meet once a piece); with more, each half has
+//     its MMA.  An 8x8 transpose of f16 pairs (movmatrix) turns the score
+//     fragment into that operand;
+//   - what must not exceed f16 is weight times scale, so the running reference
+//     is that of the products: with H the largest exponent of a V scale in the
+//     piece so far and e_t a token's, m is the largest z_t + e_t - H, weights
+//     are 2^(z_t - m), and the operand is a weight times v_scale 2^(15 - H).
+//     A row's largest product is above 2^14 there, whatever blocks of larger
+//     scale but no weight lie beside it, and a token is off by at most 2^-25,
+//     2^-39 of that largest product;
+//   - e_t - H counts as -100 below that, so that weights stay within float32
+//     (2^100 at most).  When H rises by d, m falls by d (by less where a block
+//     is already 100 below H): the producer, which sees the scales in order,
+//     adds these up.  So blocks of one sequence lose nothing to one another
+//     while their scales are within 2^100; a scale further below the largest
+//     one keeps as many bits less;
+//   - m is rounded up to a whole number: all factors between references are
+//     then exact powers of two;
 //   - the value sum of a pass (64 tokens; 32 for head_dim 256) starts from zero
 //     in the tensor cores and is added to f32 registers, so the chain of
 //     truncated tensor-core additions is four long (eight where each half has
@@ -77,6 +87,15 @@ struct Fp8Args : DecodeArgs {
 };
 
 constexpr int kSclRing = 128;  // slices whose scales the ring holds (see fp8_produce)
+
+// What the consumers need of a slice's scales (see the top).
+struct __align__(16) SliceScales {
+  float k;       // K scale
+  float v;       // V scale * 2^(15 - H)
+  float rel;     // the V scale's exponent less H, -kSpan at least
+  int units;     // H, and above it the sum of what it lowers m by
+};
+constexpr int kSpan = 100;
 
 // Stage tokens: 16 KB of K and V.
 constexpr int stage_tokens(int head_dim) { return 8192 / head_dim; }
@@ -328,6 +347,11 @@ __device__ __noinline__ bool slot_wait(uint32_t bar, uint32_t parity, volatile i
   return false;
 }
 
+// e with x < (2 - 2^-10) 2^e, so that 2^15 x 2^-e stays within f16; -126 <= e <= 127.
+__device__ __forceinline__ int scale_exponent(float x) {
+  return min(max((__float_as_int(x) + 0x2000) >> 23, 1), 254) - 127;
+}
+
 // The producer warp (produce() of decode_common.cuh for this cache): walks
 // the CTA's range, posts each piece, appends the new token where the piece
 // ends its sequence, and streams the slices.
@@ -341,7 +365,7 @@ __device__ __noinline__ bool slot_wait(uint32_t bar, uint32_t parity, volatile i
 // group is written when at most nstage stages are unconsumed, so nstage * sb +
 // 32 <= kSclRing entries are live.
 template <typename T, int D>
-__device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* map, const SmemPtrs& sm, const SmemPlan& sp, float2* scl,
+__device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* map, const SmemPtrs& sm, const SmemPlan& sp, SliceScales* scl,
                             int sb, const WalkStart& ws) {
   constexpr int RPT = D >= 128 ? D / 128 : 1;  // rows of the copies' tensor map per token
   const int lane = threadIdx.x & 31, sub_shift = a.real_shift - a.slice_shift;
@@ -384,6 +408,7 @@ __device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* map, const Smem
   };
 
   const int alpha = a.seg_cost, sb_shift = 31 - __clz(sb);
+  int vmax = 0, vmin = 0, lowered = 0;  // the piece's V exponents so far
 
   int b = ws.b, h = ws.h, off = ws.off, npiece = 0;
   int left = (int)(ws.hi - ws.lo);  // stream positions of the range still to walk
@@ -493,7 +518,30 @@ __device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* map, const Smem
       const int n = min(32, x.nblk - j0);  // slices of this group
       const bool final = j0 + 32 >= x.nblk;
       const int issued = cur.row;
-      scl[(stage * sb + lane) & (kSclRing - 1)] = make_float2(cur.sk, cur.sv);
+      {
+        // behind the piece: its last slice once more
+        const float sk = __shfl_sync(0xffffffffu, cur.sk, min(lane, n - 1));
+        const float sv = __shfl_sync(0xffffffffu, cur.sv, min(lane, n - 1));
+        const int e = scale_exponent(sv);
+        const int hi = __reduce_max_sync(0xffffffffu, e), lo = __reduce_min_sync(0xffffffffu, e);
+        if (j0 == 0) {
+          vmax = hi;
+          vmin = lo;
+          lowered = 0;
+        } else {
+          const int was = min(vmax - vmin, kSpan);
+          vmax = max(vmax, hi);
+          lowered += min(vmax - vmin, kSpan) - was;
+          vmin = min(vmin, lo);
+        }
+        SliceScales f;
+        f.k = sk;
+        // (2^(15 - H) in two factors: it may be above 2^127)
+        f.v = sv * __int_as_float((127 + min(15 - vmax, 127)) << 23) * __int_as_float((127 + max(15 - vmax - 127, 0)) << 23);
+        f.rel = (float)max(e - vmax, -kSpan);
+        f.units = lowered * 256 + vmax + 128;
+        scl[(stage * sb + lane) & (kSclRing - 1)] = f;
+      }
       __syncwarp();
       if (final) {
         have2 = claim(x2);
@@ -681,7 +729,8 @@ __device__ __forceinline__ int v_unit(int g, int p) {
   return D == 64 ? g : 2 * ((g & 1) + 2 * p + 4 * (g >> 2)) + ((g >> 1) & 1);
 }
 
-// 2^x; the hardware's, flushing results below 2^-126.
+// 2^x; the hardware's, flushing results below 2^-126.  Exact for whole x (all
+// of -126 .. 127 tried on the GPU).
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -723,7 +772,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 __device__ __forceinline__ float floor_pow2(float x) {
   return __int_as_float(min(max(__float_as_int(x) & 0x7f800000, 1 << 23), 252 << 23));
 }
-__device__ __forceinline__ float inv_pow2(float x) { return __int_as_float((254 << 23) - __float_as_int(x)); }
 
 // kShaped: scores may be capped or biased; kKept: they are written out for the
 // weights; kTwin: groups of up to 4 queries.  A variant has none of the others'
@@ -749,7 +797,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
   const SmemPlan sp = smem_plan(vs, D, 1, sb, a.nstage, (NCW - 1) * group * S * (int)sizeof(float),
                                 group * D * (int)sizeof(T), 1);
   const SmemPtrs sm = smem_ptrs(smem, sp, a.nstage);
-  float2* scl = reinterpret_cast<float2*>(reinterpret_cast<unsigned char*>(sm.scratch) + sp.scratch_bytes);
+  SliceScales* scl = reinterpret_cast<SliceScales*>(reinterpret_cast<unsigned char*>(sm.scratch) + sp.scratch_bytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) prefetch_tensor_map(&map);
   init_barriers<1, NCW - 1>(sm, a.nstage, NCW);
@@ -833,7 +881,8 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
     float* zrow =
         kKept ? a.z + ((size_t)(x.b * a.num_kv_heads + x.h) * group + 2 * tq) * a.z_stride : nullptr;
 
-    float m[2] = {-INFINITY, -INFINITY}, vref = 0.f;
+    float m[2] = {-INFINITY, -INFINITY};
+    int units = 128;  // of the passes so far (SliceScales)
     float2 l2 = make_float2(0.f, 0.f);
     // value sums: o[4 i + k] is dim k (of 4) of half i of this lane's V units, queries 2 tq and 2 tq + 1
     float2 o[D / 8];
@@ -867,8 +916,8 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
       for (int p0 = 0; p0 < (TT == PT ? 1 : hi); p0 += PT) {
         // ---- scores: tile e is tokens p0 + 8 e + g, queries 2 tq + c ----
         float2 z[NE];
-        float wv[NE];
-        float vmax = 0.f;
+        int now = 0;
+        float wv[NE], rel[NE];
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
           uint4 kw[2][KJ];
@@ -896,9 +945,10 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const int e = 2 * k + r;
-            const uint2 f = lds64(sbase + ((s_first + ((p0 + 8 * e) >> vshift)) & (kSclRing - 1)) * 8);
+            const uint4 f = lds128(sbase + ((s_first + ((p0 + 8 * e) >> vshift)) & (kSclRing - 1)) * 16);
             wv[e] = __uint_as_float(f.y);
-            vmax = fmaxf(vmax, wv[e]);
+            rel[e] = __uint_as_float(f.z);
+            if (e == 0) now = (int)f.w;
             z[e] = mul2(make_float2(s[2 * r], s[2 * r + 1]), mul2(both(__uint_as_float(f.x)), zf));
           }
         }
@@ -948,35 +998,41 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
           }
         }
         // ---- online softmax of queries 2 tq and 2 tq + 1 ----
-        const float vnew = fmaxf(vref, floor_pow2(vmax)), vinv = inv_pow2(vnew);
-        float corr[2], ms[2];
+        const float lowered = (float)((now >> 8) - (units >> 8)), down = ex2((float)((units & 255) - (now & 255)));
+        units = now;
+        float corr[2], oc[2];
+        float2 top = add2(z[0], both(rel[0]));
+#pragma unroll
+        for (int e = 1; e < NE; ++e) {
+          const float2 t = add2(z[e], both(rel[e]));
+          top = make_float2(fmaxf(top.x, t.x), fmaxf(top.y, t.y));
+        }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float mx = c ? z[0].y : z[0].x;
-#pragma unroll
-          for (int e = 1; e < NE; ++e) mx = fmaxf(mx, c ? z[e].y : z[e].x);
+          float mx = c ? top.y : top.x;
 #pragma unroll
           for (int s = 4; s < 32; s <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
-          const float mn = fmaxf(m[c], mx);
-          ms[c] = mn == -INFINITY ? 0.f : 14.f - mn;
-          corr[c] = m[c] == -INFINITY ? 0.f : ex2(m[c] - mn);
+          const float mn = fmaxf(m[c] - lowered, ceilf(mx));
+          const float up = fmaxf(m[c] - mn, -1024.f);  // (also where both are -infinity)
+          corr[c] = ex2(up);
+          oc[c] = corr[c] * down;
           m[c] = mn;
         }
+        const float2 ms = make_float2(m[0] == -INFINITY ? 0.f : -m[0], m[1] == -INFINITY ? 0.f : -m[1]);
         l2 = mul2(l2, make_float2(corr[0], corr[1]));
         // the P^T operand (tokens x queries): both halves of the weights, or, where columns 4..7 repeat the queries,
         // the high halves in columns 0..3 and the low ones in 4..7
         uint32_t ph[NE], pl[kTwin ? 1 : NE];
 #pragma unroll
         for (int e = 0; e < NE; ++e) {
-          const float2 d = add2(z[e], make_float2(ms[0], ms[1])), w = make_float2(ex2(d.x), ex2(d.y));
+          const float2 d = add2(z[e], ms), w = make_float2(ex2(d.x), ex2(d.y));
           l2 = add2(l2, w);
           uint32_t hi2, lo2;
-          split_halves(mul2(w, both(wv[e] * vinv)), hi2, lo2);
+          split_halves(mul2(w, both(wv[e])), hi2, lo2);
           ph[e] = transpose8x8(kTwin && tq >= 2 ? lo2 : hi2);
           if constexpr (!kTwin) pl[e] = transpose8x8(lo2);
         }
-        const float2 oc = mul2(make_float2(corr[0], corr[1]), both(vref * vinv));
-        vref = vnew;
+        const float2 oc2 = make_float2(oc[0], oc[1]);
         // ---- value sum, V^T (16 dims) times P^T (8 queries) ----
 #pragma unroll
         for (int u = 0; u < VH * VP; ++u) {
@@ -1016,7 +1072,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
                 float2& on = o[(u * 2 + w) * 4 + 2 * i + r];
-                on = fma2(on, oc, make_float2(d[i][2 * r], d[i][2 * r + 1]));
+                on = fma2(on, oc2, make_float2(d[i][2 * r], d[i][2 * r + 1]));
               }
           }
         }
@@ -1029,20 +1085,28 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
     gbase += x.nstages;
 
     // ---- hand-off: the last warp to finish a piece merges the others' states
-    // (acc, m - 14, l), left in scratch, with its own, still in registers.
+    // (acc, M, l), left in scratch, with its own, still in registers: acc and l
+    // sums of 2^(z - M) v and 2^(z - M), M whole and such that 1 <= l < 2 (or 0).
     // Lane (g, tq) holds queries 2 tq and 2 tq + 1 of its V units' dims. ----
     float l[2] = {l2.x, l2.y};
+    float2 unit;
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int c = 0; c < 2; ++c) {
 #pragma unroll
       for (int s = 4; s < 32; s <<= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], s);
+      // (o is in units of 2^(H - 15); less is taken off l where that, less k, would leave float32)
+      const int h = (units & 255) - 128, k = max(min((__float_as_int(l[c]) >> 23) - 127, h + 111), -15);
+      l[c] *= __int_as_float((127 - k) << 23);
+      m[c] += (float)k;
+      (c ? unit.y : unit.x) = __int_as_float((127 + h - 15 - k) << 23);
+    }
     if constexpr (kTwin) {  // high and low halves' sums
 #pragma unroll
       for (int n = 0; n < D / 8; ++n)
         o[n] = add2(o[n], make_float2(__shfl_xor_sync(0xffffffffu, o[n].x, 2), __shfl_xor_sync(0xffffffffu, o[n].y, 2)));
     }
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n) o[n] = mul2(o[n], both(vref));
+    for (int n = 0; n < D / 8; ++n) o[n] = mul2(o[n], unit);
     auto sum = [&](int n, int c) { return c ? o[n].y : o[n].x; };
     const uint32_t par = (uint32_t)n_done & 1u;
     if (!wait_or_abort(a, sm, &sm.scr_empty[0], par ^ 1u)) return;
@@ -1064,7 +1128,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
                 make_float4(sum(4 * i, c), sum(4 * i + 1, c), sum(4 * i + 2, c), sum(4 * i + 3, c));
         }
         if (g == 0) {
-          row[D] = m[c] - 14.f;
+          row[D] = m[c];
           row[D + 1] = l[c];
           row[D + 2] = (float)cw;
         }
@@ -1093,7 +1157,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
           const float po = __fmul_rn(wo, xo), pb = __fmul_rn(wb, xb);
           return __fadd_rn(__fadd_rn(own_last ? pb : po, __fmul_rn(wa, xa)), own_last ? po : pb);
         };
-        const float mo = m[c] - 14.f, M = fmaxf(mo, fmaxf(A[D], B[D]));
+        const float mo = m[c], M = fmaxf(mo, fmaxf(A[D], B[D]));
         const float fo = mo == -INFINITY ? 0.f : ex2(mo - M);
         const float fa = A[D] == -INFINITY ? 0.f : ex2(A[D] - M), fb = B[D] == -INFINITY ? 0.f : ex2(B[D] - M);
         const float L = add(fo, l[c], fa, A[D + 1], fb, B[D + 1]);
@@ -1379,7 +1443,7 @@ static int fp8_cfg(const clove_fp8_pool& pool, int slice, int group, Fp8Cfg* out
   Fp8Cfg c;
   const int stage = smem_plan(slice, D, 1, sb, 1, scratch, qb, 1).stage_bytes;
   auto bytes = [&](int n) {
-    return smem_plan(slice, D, 1, sb, n, scratch, qb, 1).total + kSclRing * (int)sizeof(float2) + 1024;
+    return smem_plan(slice, D, 1, sb, n, scratch, qb, 1).total + kSclRing * (int)sizeof(SliceScales) + 1024;
   };
   // as deep a ring as two CTAs on an SM leave room for
   c.nstage = std::max(1, ring / stage / kFp8Warps) * kFp8Warps;

@@ -21,7 +21,10 @@
  * by the same call hold nothing.  So blocks are filled from row 0 on, as the
  * block manager's tables do.  Infinities are stored as +-448 * scale, NaN as
  * NaN; neither counts towards a scale.  Scales written by other means (a
- * loaded cache) may be any positive finite number.
+ * loaded cache) may be any positive number up to 2^127.  A decode's outputs
+ * are as exact as float32 weights make them while the V scales of a sequence
+ * and KV head are within 2^100 of one another; a block whose scale is further
+ * below the largest one keeps as many bits less.
  *
  * Shapes: head_dim 64, 128 or 256; block_size a power of two in [8, 256];
  * num_q_heads / num_kv_heads in 1..8.  q, k, v and the new token may be f32,

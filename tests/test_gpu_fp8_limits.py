@@ -1,0 +1,122 @@
+"""The 8-bit cache at the ends of its range: sequences that the partition
+splits, blocks far into a large cache, scales and values of any size, calls
+that run into their wait limit, and what is refused.
+
+Outputs are held to sharp_bound, which knows no scale but those that matter:
+a block of negligible weight may not cost another one precision.
+"""
+import ctypes as C
+
+import pytest
+import torch
+
+from clove_b200 import _lib
+from fp8_reference import RefPool
+from test_gpu_fp8 import DEV, F8, i32, make_pool, run_decode, tables_for
+
+pytestmark = pytest.mark.gpu
+
+# ---------------------------------------------------------------------------
+# scales of any size
+# ---------------------------------------------------------------------------
+def sharp_bound(ref, q, tables, lens, scale):
+    """(out, bound) in 64 bits for a float32 computation of plain scores.
+
+    Token t's score is a float32 sum of D products, rounded or truncated at
+    most D / 16 + 8 times, so off by at most e_t = (D / 16 + 8) 2^-23 S_t, S_t
+    its sum of magnitudes; exp2, the two halves of a weight and the sums over L
+    tokens add c = (L / 32 + 24) 2^-23.  A weight p_t is thus off by p_t (e_t +
+    c) in the numerator, and the denominator by the sum of these.  What a
+    weight times its block's scale s_t falls below f16's smallest step is
+    rounded at 2^-25 in units in which the largest such product of the row is
+    at least 2^10: 2^-35 max(p s) |code_t| for each token."""
+    q = q.cpu().double()
+    B, hq, D = q.shape
+    H = ref.codes.shape[2]
+    out, bound = torch.zeros(B, hq, D, dtype=torch.float64), torch.zeros(B, hq, D, dtype=torch.float64)
+    for b in range(B):
+        L = int(lens[b])
+        pos = torch.arange(L)
+        k, v = (ref.rows(p, tables[b].cpu(), pos) for p in range(2))
+        blk = tables[b].cpu().long()[pos // ref.bs]
+        for h in range(H):
+            g = slice(h * (hq // H), (h + 1) * (hq // H))
+            z = scale * q[b, g] @ k[:, h].t()
+            e = (D / 16 + 8) * 2.0 ** -23 * (abs(scale) * q[b, g].abs() @ k[:, h].abs().t()) + (L / 32 + 24) * 2.0 ** -23
+            p = torch.softmax(z, 1)
+            out[b, g] = p @ v[:, h]
+            mag = v[:, h].abs()
+            top = (p * ref.scales[1][blk, h]).amax(1)
+            bound[b, g] = (p * e) @ mag + (p * e).sum(1, keepdim=True) * (p @ mag) + 1e-37 + \
+                2.0 ** -35 * top[:, None] * ref.codes[1][blk, h, pos % ref.bs].abs().sum(0)
+    return out, bound
+
+
+def levels(lens, bs, H, G, D, dtype, seed, size, weight):
+    """A pool of sequences whose block j holds values of about 2^size(j) and
+    scores of about weight(j) in the log2 domain, and what a decode of it gives."""
+    from clove_b200 import Fp8KVPool
+    gen = torch.Generator().manual_seed(seed)
+    tables, nb = tables_for(lens, bs, gen)
+    pool = Fp8KVPool(nb, bs, H, D)
+    for b, n in enumerate(lens):
+        t = torch.arange(n)
+        blocks = [int(x) for x in t // bs]
+        k, v = torch.randn((n, H, D), generator=gen) * 0.05, torch.randn((n, H, D), generator=gen)
+        k[:, :, 0] = torch.tensor([float(weight(j)) for j in blocks])[:, None]
+        v *= torch.tensor([2.0 ** size(j) for j in blocks])[:, None, None]
+        slots = tables[b].cpu().long()[t // bs] * bs + t % bs
+        pool.reshape_and_cache(k.to(DEV), v.to(DEV), i32(slots))
+    ref = RefPool(pool.storage, pool.scales)
+    q = (torch.randn((len(lens), H * G, D), generator=gen) * 0.5).to(dtype)
+    q[:, :, 0] = 1.0
+    scale = 0.6931471805599453  # scores in the log2 domain
+    want, bound = sharp_bound(ref, q, tables, lens, scale)
+    out = pool.decode(q.to(DEV), tables, i32(lens), scale=scale, max_ctx=max(lens))
+    assert pool.pool_status() == 0
+    err = (out.cpu().double() - want).abs()
+    assert (err <= bound).all(), f"{float((err / bound).max()):.3g} of the bound"
+
+
+SHAPES = [(torch.bfloat16, 16, 2, 4, 128), (torch.float16, 8, 2, 8, 64), (torch.float32, 32, 1, 1, 256),
+          (torch.float32, 64, 1, 8, 128), (torch.bfloat16, 256, 1, 2, 64), (torch.float16, 128, 1, 6, 256)]
+
+
+@pytest.mark.parametrize("dtype,bs,H,G,D", SHAPES)
+@pytest.mark.parametrize("ratio", [3, 6, 26, 40, 100])
+@pytest.mark.parametrize("at", ["first", "middle", "last"])
+def test_a_loud_block_of_no_weight(dtype, bs, H, G, D, ratio, at):
+    # one block's values are 2^ratio times the others', its tokens weigh nothing
+    for lens in ([3 * bs + 5, 700], [9 * bs + 1, 6000]):
+        for n in lens:
+            last = (n - 1) // bs
+            j0 = {"first": 0, "middle": (last + 1) // 2, "last": last}[at]
+            levels([n], bs, H, G, D, dtype, ratio + n, lambda j: ratio if j == j0 else 0, lambda j: -220 if j == j0 else 0)
+
+
+@pytest.mark.parametrize("dtype,bs,H,G,D", SHAPES)
+@pytest.mark.parametrize("ratio", [6, 26, 60, 100])
+def test_loud_blocks_of_little_weight(dtype, bs, H, G, D, ratio):
+    # every other block's values are 2^ratio times the others', its tokens' weights as much smaller: they count alike
+    levels([700, 9 * bs + 1], bs, H, G, D, dtype, ratio, lambda j: ratio * (j & 1), lambda j: -ratio * (j & 1))
+    levels([4000], bs, H, G, D, dtype, ratio, lambda j: -ratio * (j & 1), lambda j: ratio * (j & 1))
+
+
+@pytest.mark.parametrize("dtype,bs,H,G,D", SHAPES)
+@pytest.mark.parametrize("slope", [-2.0, -1.0, -0.5, 0.0, 1.0])
+@pytest.mark.parametrize("way", [1, -1])
+def test_scales_in_steps(dtype, bs, H, G, D, slope, way):
+    # values grow or shrink from block to block over 2^120, weights with slope times that
+    n = 24 * bs - 3
+    levels([n], bs, H, G, D, dtype, 5, lambda j: way * (5 * j - 60), lambda j: slope * way * (5 * j - 60))
+
+
+@pytest.mark.parametrize("dtype,bs,H,G,D", SHAPES)
+def test_scales_of_each_kv_head_and_query_apart(dtype, bs, H, G, D):
+    # random sizes and weights, independent of one another
+    gen = torch.Generator().manual_seed(1)
+    size = torch.randint(-50, 50, (800,), generator=gen).tolist()
+    weight = (torch.randn((800,), generator=gen) * 40).tolist()
+    levels([900, 5000, 17], bs, H, G, D, dtype, 6, lambda j: size[j], lambda j: weight[j])
+
+
