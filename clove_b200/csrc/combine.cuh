@@ -152,6 +152,12 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const Args a) 
       *a.err = 0;
     }
   }
+  // did any CTA of the decode give up on a wait? (asked here, told below)
+  int gave_up = 0;
+  if constexpr (Args::kKeepsRowState) {
+    if (blockIdx.x == 0 && a.gave_up != nullptr)
+      for (int i = threadIdx.x; i < a.num_ctas; i += kCombineThreads) gave_up |= __ldcg(a.gave_up + i);
+  }
   const long long W = *a.total;
   const long long P = a.num_ctas;
   const int alpha = a.seg_cost;
@@ -195,6 +201,12 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const Args a) 
     const int o_begin = (int)((long long)helper * n_out / helpers);
     const int o_end = (int)((long long)(helper + 1) * n_out / helpers);
     combine_segment<D, Args>(a, d.x, d.y, pieces, np, pm, pl, run, rowv, o_begin, o_end);
+  }
+  if constexpr (Args::kKeepsRowState) {
+    if (blockIdx.x == 0 && a.gave_up != nullptr) {
+      gave_up = __syncthreads_or(gave_up);
+      if (threadIdx.x == 0) a.gave_up[a.num_ctas] = gave_up;
+    }
   }
   if constexpr (kTrace) {
     if (a.trace && threadIdx.x == 0) atomicMax(a.trace + 3, gtime());

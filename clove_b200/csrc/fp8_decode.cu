@@ -77,6 +77,7 @@ struct Fp8Args : DecodeArgs {
   float2* row_state;   // [batch, Hq]: (M, 1 / L) of each output row (accumulate only, else null)
   float* z;            // [batch, Hq, z_stride]: scores in the log2 domain (accumulate only, else null)
   long long z_stride;
+  int* gave_up;        // [num_ctas + 1]: CTAs that gave up on a wait, then whether any did (accumulate only, else null)
   int real_block;      // tokens per cache block; DecodeArgs::block_size is the slice
   int slice_shift;     // log2 of the slice
   int real_shift;      // log2 of real_block
@@ -114,6 +115,7 @@ __device__ __noinline__ unsigned long long udiv64(unsigned long long a, unsigned
 template <int D>
 __device__ void fp8_prologue(const Fp8Args& a, WalkStart* out) {
   const int tid = threadIdx.x, lane = tid & 31, nt = blockDim.x, H = a.num_kv_heads;
+  if (tid == 0 && a.gave_up != nullptr) a.gave_up[blockIdx.x] = 0;
   if (a.direct) {
     const int b = blockIdx.x / H, h = blockIdx.x - b * H;
     const int raw = __ldg(a.context_lens + b);
@@ -272,7 +274,7 @@ __device__ __forceinline__ void fp8_store_new(const Fp8Args& a, int h, int L, in
     dst[i / 4] = fp8_pack2(n.v[i] * inv, n.v[i + 1] * inv) | fp8_pack2(n.v[i + 2] * inv, n.v[i + 3] * inv) << 16;
   if ((lane & 15) == 0) a.scales[(size_t)p * a.num_blocks * H + tile] = s;
   n.old = s;
-  if (lane == 0 && a.mass != nullptr && a.z == nullptr) a.mass[tile * bs + off] = 0.f;
+  if (lane == 0 && a.mass != nullptr) a.mass[tile * bs + off] = 0.f;
   fence_proxy_async_global();
   __syncwarp();
 }
@@ -599,6 +601,7 @@ __device__ void fp8_produce(const Fp8Args& a, const CUtensorMap* map, const Smem
     x = x2;
   }
   if (aborted && lane == 0) {
+    if (a.gave_up != nullptr) a.gave_up[blockIdx.x] = 1;
     // drain: the last nstage stages and unit posts may still be in flight
     int s = slot;  // 1 .. nstage: the slot behind the last one issued
     uint32_t ph = phase;
@@ -1081,7 +1084,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.empty[slot]);
     }
-    if (aborted) return;  // the abort flag is up; every other warp leaves at its next wait
+    if (aborted) break;  // the abort flag is up; every other warp leaves at its next wait
     gbase += x.nstages;
 
     // ---- hand-off: the last warp to finish a piece merges the others' states
@@ -1109,7 +1112,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
     for (int n = 0; n < D / 8; ++n) o[n] = mul2(o[n], unit);
     auto sum = [&](int n, int c) { return c ? o[n].y : o[n].x; };
     const uint32_t par = (uint32_t)n_done & 1u;
-    if (!wait_or_abort(a, sm, &sm.scr_empty[0], par ^ 1u)) return;
+    if (!wait_or_abort(a, sm, &sm.scr_empty[0], par ^ 1u)) break;
     int order = 0;
     if (lane == 0) {
       order = atomicAdd(&sm.arrive[0], 1);
@@ -1136,7 +1139,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.scr_empty[1]);  // [1]: the others' states are in scratch
     } else {
-      if (!wait_or_abort(a, sm, &sm.scr_empty[1], par)) return;
+      if (!wait_or_abort(a, sm, &sm.scr_empty[1], par)) break;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int q = 2 * tq + c;
@@ -1198,20 +1201,22 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
       uphase ^= 1;
     }
   }
+  if (kKept && sm.misc[0] && lane == 0) a.gave_up[blockIdx.x] = 1;
 }
 
 // ---------------------------------------------------------------------------
 // weights: mass += sum over the group of 2^(z - M) / L
 // ---------------------------------------------------------------------------
-constexpr int kMassThreads = 256, kMassCtas = 8;  // CTAs per SM
+constexpr int kMassThreads = 256, kMassCtas = 6;  // CTAs per SM, all resident
 constexpr int kMassTokens = 128;                  // tokens per warp and step: four per lane
 
 // The steps of all (sequence, KV head) pairs are one stream, sequence by
 // sequence, and every warp takes an equal run of it: with lengths that differ
 // the longest sequence would otherwise hold its warps several times as long as
 // the others theirs (128 ragged sequences: 4 us more).  Bound by latency: the
-// scores come from L2 where they fit it, and a warp has one or two steps.
-__global__ void __launch_bounds__(kMassThreads) fp8_mass_kernel(const Fp8Args a) {
+// scores come from L2 where they fit it, and a warp has one or two steps; CTAs
+// in a second wave cost 3 us there.
+__global__ void __launch_bounds__(kMassThreads, kMassCtas) fp8_mass_kernel(const Fp8Args a) {
   constexpr int kWarps = kMassThreads / 32;
   __shared__ int warp_tot[kWarps], start[kMassThreads], count[kMassThreads];
   __shared__ long long s_rest;
@@ -1270,7 +1275,16 @@ __global__ void __launch_bounds__(kMassThreads) fp8_mass_kernel(const Fp8Args a)
     before = block_excl_scan(n, warp_tot, &tot);
   }
   griddep_wait();  // (the lengths were complete before the decode let this kernel be launched)
+  // Where a CTA of the decode gave up, scores and row states are not what they
+  // should be: the call then adds no weights at all, so that it can be repeated.
   if (b < 0) return;
+  int gave_up = 0;
+  if (a.direct) {
+    for (int i = lane; i < a.num_ctas; i += 32) gave_up |= __ldcg(a.gave_up + i);
+    gave_up = __any_sync(0xffffffffu, gave_up);
+  } else {
+    gave_up = __ldcg(a.gave_up + a.num_ctas);  // the combine has looked through them
+  }
   int L = clamp_ctx(a.context_lens, b, a.max_ctx, a.append);
   for (; left > 0; --left, ++c) {
     if (c == len) {  // the next KV head, or the next sequence that has tokens
@@ -1301,6 +1315,7 @@ __global__ void __launch_bounds__(kMassThreads) fp8_mass_kernel(const Fp8Args a)
       w[2] = fmaf(ex2(v.z - st.x), st.y, w[2]);
       w[3] = fmaf(ex2(v.w - st.x), st.y, w[3]);
     }
+    if (gave_up) return;  // (not before: the word arrives beside the scores)
     // added atomically: forked sequences share blocks
     if (t >= t0 && t + 4 <= L - a.append) {
       asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(dst), "f"(w[0]), "f"(w[1]), "f"(w[2]), "f"(w[3])
@@ -1333,10 +1348,13 @@ static int fp8_segment_cost(int slice, int head_dim) {
   return (40 * 1024 + bytes - 1) / bytes;
 }
 
+// The most (sequence, KV head) pairs that are taken whole (fp8_direct).
+static int direct_ctas(const clove_fp8_pool& pool) { return 4 * pool.num_sms; }
+
 struct Fp8Layout {
   int max_ctas;
   long long z_stride;
-  size_t off_total, off_desc, off_partials, off_rows, off_z, total;
+  size_t off_total, off_desc, off_partials, off_gave_up, off_rows, off_z, total;
 };
 
 static Fp8Layout fp8_layout(const clove_fp8_pool& pool, int batch, int num_q_heads, int max_ctx, int accumulate) {
@@ -1348,10 +1366,10 @@ static Fp8Layout fp8_layout(const clove_fp8_pool& pool, int batch, int num_q_hea
   L.off_total = 0;
   L.off_desc = 256;
   L.off_partials = up(L.off_desc + sizeof(int4) * (size_t)L.max_ctas);
-  L.off_rows = up(L.off_partials + sizeof(float) * (size_t)L.max_ctas * 2 * group * state_stride(pool.head_dim));
-  L.off_z = L.off_rows;
-  L.total = L.off_rows;
+  L.off_gave_up = up(L.off_partials + sizeof(float) * (size_t)L.max_ctas * 2 * group * state_stride(pool.head_dim));
+  L.off_rows = L.off_z = L.total = L.off_gave_up;
   if (accumulate) {
+    L.off_rows = up(L.off_gave_up + sizeof(int) * (size_t)std::max(L.max_ctas + 1, direct_ctas(pool)));
     L.off_z = up(L.off_rows + sizeof(float2) * (size_t)batch * num_q_heads);
     L.total = up(L.off_z + sizeof(float) * (size_t)batch * num_q_heads * L.z_stride);
   }
@@ -1365,7 +1383,7 @@ static Fp8Layout fp8_layout(const clove_fp8_pool& pool, int batch, int num_q_hea
 // 18.5 / 37.1 against 22.3 / 40.0; 128 of 100 / 1000: 32.9 / 71.6 against 28.8
 // / 60.8, since the CTAs then come in more than two waves.
 static bool fp8_direct(const clove_fp8_pool& pool, int batch, int longest) {
-  return (long long)batch * pool.num_kv_heads <= 4LL * pool.num_sms && longest <= kDirectTokens;
+  return (long long)batch * pool.num_kv_heads <= direct_ctas(pool) && longest <= kDirectTokens;
 }
 
 size_t fp8_decode_workspace(const clove_fp8_pool& pool, int batch, int num_q_heads, int max_ctx, int accumulate) {
@@ -1568,6 +1586,7 @@ int launch_fp8_decode(const clove_fp8_pool& pool, const Fp8DecodeCall& c, cudaSt
   a.softcap = c.scores.softcap;
   if (c.scores.accumulate) {
     a.row_state = reinterpret_cast<float2*>(ws + L.off_rows);
+    a.gave_up = reinterpret_cast<int*>(ws + L.off_gave_up);
     a.z = reinterpret_cast<float*>(ws + L.off_z);
     a.z_stride = L.z_stride;
   }

@@ -70,7 +70,8 @@ typedef struct clove_fp8_pool_info {
  * accumulate != 0: the call adds each token's attention weight, summed over
  * the query heads of its KV head, to the pool's mass (a token the call
  * appends starts at its own weight).  Sequences of one call may share blocks
- * (forks): their weights add up, in an order that may change the last bit. */
+ * (forks): their weights add up, in an order that may change the last bit.
+ * A call that gives up on a wait (CLOVE_FLAG_TIMEOUT) adds no weights. */
 typedef struct clove_fp8_scores {
     float softcap;
     const float* alibi_slopes;

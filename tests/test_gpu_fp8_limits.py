@@ -120,3 +120,44 @@ def test_scales_of_each_kv_head_and_query_apart(dtype, bs, H, G, D):
     levels([900, 5000, 17], bs, H, G, D, dtype, 6, lambda j: size[j], lambda j: weight[j])
 
 
+# ---------------------------------------------------------------------------
+# calls that run into their wait limit
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("append", [False, True])
+@pytest.mark.parametrize("bs,lens", [(16, [600, 40]), (16, [5000, 900]), (256, [5000, 900])], ids=["whole", "split", "slices"])
+def test_stuck_wait_adds_no_weights(bs, lens, append):
+    # the test hook leaves one stage unfilled: the call ends, says so, and leaves the weights as they were, but for
+    # that of the token it appends; the next call is right
+    gen = torch.Generator().manual_seed(57)
+    tables, nb = tables_for([n + 1 for n in lens], bs, gen)
+    pool = make_pool(nb, bs, 2, 128, gen, mass=True, scales=(-9, -5))
+    q = torch.randn((2, 8, 128), generator=gen)
+    kv = torch.randn((2, 2, 2, 128), generator=gen)
+    kw = dict(max_ctx=max(lens) + 1, accumulate=True)
+    if append:
+        kw |= dict(k_new=kv[0].to(DEV), v_new=kv[1].to(DEV))
+    before = pool.mass.clone()
+    torch.full((1 << 26,), float("nan"), device=DEV)  # what the allocator gives as scratch next
+    L = _lib.lib()
+    torch.cuda.synchronize()
+    try:
+        _lib.check(L.clove_cuda_debug_set(2000, 1))
+        pool.decode(q.to(DEV), tables, i32(lens), **kw)
+        assert pool.pool_status() & _lib.FLAG_TIMEOUT
+    finally:
+        L.clove_cuda_debug_set(0, 0)
+    if append:
+        for b, n in enumerate(lens):
+            before[int(tables[b, n // bs]), :, n % bs] = pool.mass[int(tables[b, n // bs]), :, n % bs]
+    assert torch.equal(pool.mass, before)
+    pool.reshape_and_cache(kv[0].to(DEV), kv[1].to(DEV), i32([int(tables[b, n // bs]) * bs + n % bs for b, n in enumerate(lens)]))
+    ref = RefPool(pool.storage, pool.scales, pool.mass)
+    if append:
+        ref.append(kv[0], kv[1], torch.tensor([int(tables[b, n // bs]) * bs + n % bs for b, n in enumerate(lens)]))
+    want, bound = ref.decode(q, tables, [n + append for n in lens], 128 ** -0.5, accumulate=True)
+    out = pool.decode(q.to(DEV), tables, i32(lens), **kw)
+    assert pool.pool_status() == 0
+    assert ((out.cpu().double() - want).abs() <= bound).all()
+    assert ((pool.mass.cpu().double() - ref.mass).abs() <= ref.mass_bound).all()
+
+
