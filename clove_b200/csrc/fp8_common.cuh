@@ -4,6 +4,8 @@
 
 #include <cuda_fp8.h>
 
+#include <mutex>
+
 #include "../../include/clove_fp8.h"
 #include "common.cuh"
 #include "host.h"
@@ -19,7 +21,8 @@ struct clove_fp8_pool {
   float* scales;         // [2, num_blocks, num_kv_heads]
   float* mass;           // [num_blocks, num_kv_heads, block_size] or null
   size_t plane_bytes;    // bytes of one plane of codes
-  int32_t* flags;        // device word: check flags of all calls
+  int32_t* flags;        // device words: check flags of all calls; those that the last status call took off
+  std::mutex status_lock;  // held while a status call takes flags off
   int32_t* slot_token;   // append index: a word per slot, then one per block; zero between calls
   int num_sms;
   CUtensorMap map;  // the codes as the decode's copies see them

@@ -92,6 +92,9 @@ int finish_pool(clove_fp8_pool* p) {
   return fp8_encode_map(*p);
 }
 
+// Takes the flags off in one step: calls on other streams may be raising some.
+__global__ void take_flags_kernel(int32_t* flags, int32_t* taken) { *taken = atomicExch(flags, 0); }
+
 // Tables, lengths and bounds that every reading call takes.
 int check_tables(const clove_fp8_pool* pool, const char* who, const int32_t* block_tables, int bt_stride,
                  const int32_t* context_lens, int batch, int max_ctx) {
@@ -214,13 +217,20 @@ int clove_fp8_pool_info(clove_fp8_pool_t pool, clove_fp8_pool_info_t* info) {
 int clove_fp8_pool_status(clove_fp8_pool_t pool, void* stream, int* flags) {
   if (!pool) return fail(CLOVE_ERR_INVALID_ARG, "fp8_pool_status: null pool");
   OnDevice g(pool->device);
+  if (!g.ok) return cuda_fail("cudaSetDevice", cudaGetLastError());
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int host = 0;
-  cudaError_t e = cudaMemcpyAsync(&host, pool->flags, sizeof(int), cudaMemcpyDeviceToHost, s);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-  if (e == cudaSuccess) e = cudaMemsetAsync(pool->flags, 0, sizeof(int), s);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-  if (e != cudaSuccess) return cuda_fail("fp8_pool_status", e);
+  try {
+    const std::lock_guard<std::mutex> lk(pool->status_lock);  // the word taken off is one per pool
+    take_flags_kernel<<<1, 1, 0, s>>>(pool->flags, pool->flags + 1);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaMemcpyAsync(&host, pool->flags + 1, sizeof(int), cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (e != cudaSuccess) return cuda_fail("fp8_pool_status", e);
+  } catch (const std::exception&) {
+    return fail(CLOVE_ERR_CUDA, "fp8_pool_status: lock");
+  }
+  count_launches(1);
   if (flags) *flags = host;
   if (host) {
     set_last_error("device check flags 0x%x", host);

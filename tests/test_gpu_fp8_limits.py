@@ -161,3 +161,25 @@ def test_stuck_wait_adds_no_weights(bs, lens, append):
     assert ((pool.mass.cpu().double() - ref.mass).abs() <= ref.mass_bound).all()
 
 
+# ---------------------------------------------------------------------------
+# check flags
+# ---------------------------------------------------------------------------
+def test_no_flag_is_lost_to_a_read_on_another_stream():
+    # flags raised on one stream at any time while another one's reads are under way: each is reported
+    gen = torch.Generator().manual_seed(10)
+    pool = make_pool(4, 16, 2, 64, gen)
+    kv = torch.randn((2, 1, 2, 64), generator=gen).to(DEV)
+    bad, side = i32([64]), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(400):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20000 + 173 * i)
+            pool.reshape_and_cache(kv[0], kv[1], bad)
+        seen, over = 0, False
+        while not over:
+            over = side.query()
+            seen |= pool.pool_status()
+        assert seen == _lib.FLAG_SLOT_OOB, i
+    assert pool.pool_status() == 0
+
+
