@@ -1,5 +1,6 @@
 // The C ABI of the 8-bit cache (include/clove_fp8.h): argument checks, pool
 // lifecycle and error reporting around the kernel launchers.
+#include <cfloat>
 #include <exception>
 #include <new>
 
@@ -297,7 +298,9 @@ int clove_fp8_decode(clove_fp8_pool_t pool, int dtype, const void* q, const void
   int rc = check_tables(pool, "fp8_decode", block_tables, bt_stride, context_lens, batch, max_ctx);
   if (rc) return rc;
   const clove_fp8_scores_t sc = scores ? *scores : clove_fp8_scores_t{0.f, nullptr, 0, 0};
-  if (!(sc.softcap >= 0.f) || !(sc.softcap < 3.4e38f) || sc.window < 0) {
+  // (a cap below float32's normal range has no usable inverse)
+  const bool cap_ok = sc.softcap == 0.f || (sc.softcap >= FLT_MIN && sc.softcap < 3.4e38f);
+  if (!cap_ok || sc.window < 0) {
     set_last_error("fp8_decode: softcap %g, window %d", (double)sc.softcap, sc.window);
     return CLOVE_ERR_INVALID_ARG;
   }

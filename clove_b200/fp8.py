@@ -191,6 +191,8 @@ class Fp8KVPool:
         if alibi_slopes is not None and (alibi_slopes.shape != (hq,) or alibi_slopes.dtype != torch.float32
                                          or alibi_slopes.device != self.device or not alibi_slopes.is_contiguous()):
             raise ValueError(f"alibi_slopes must be a contiguous float32 [{hq}] tensor on {self.device}")
+        if softcap and abs(softcap) < torch.finfo(torch.float32).tiny:  # float32 would make it 0, which is no cap
+            raise ValueError(f"softcap {softcap} is below float32's range")
         if accumulate and self.mass is None:
             raise ValueError("accumulate needs a pool with mass (track_mass=True)")
         shape = (batch, hq, self.head_dim)

@@ -62,7 +62,7 @@ typedef struct clove_fp8_pool_info {
 } clove_fp8_pool_info_t;
 
 /* How the decode forms a score from scale * <q, K_t>.  In this order:
- *   softcap > 0     z = softcap * tanh(z / softcap)
+ *   softcap > 0     z = softcap * tanh(z / softcap); 0, or 2^-126 at least
  *   alibi_slopes    z += alibi_slopes[hq] * (t - (L - 1)): f32 [num_q_heads]
  *                   device array or null; t the token's index in the cache,
  *                   L the tokens cached (the new one included)

@@ -183,3 +183,15 @@ def test_no_flag_is_lost_to_a_read_on_another_stream():
     assert pool.pool_status() == 0
 
 
+# ---------------------------------------------------------------------------
+# arguments
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("softcap", [1e-39, 1e-45, 1e-60, 5e-324])
+def test_caps_too_small_for_float32_are_refused(softcap):
+    # not rounded to 0, which stands for no cap
+    pool = make_pool(4, 16, 2, 64, torch.Generator().manual_seed(11))
+    with pytest.raises((ValueError, _lib.CloveError)):
+        pool.decode(torch.ones((1, 4, 64), device=DEV), i32([[0, 1]]), i32([20]), max_ctx=20, softcap=softcap)
+    assert pool.pool_status() == 0
+
+
