@@ -32,6 +32,14 @@ def _current_stream(device: int) -> int:
     return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
+# The C side takes 32 bits, to which ctypes would cut a larger number down.
+_INT_MAX = 2 ** 31 - 1
+
+
+def _fits(n: int) -> bool:
+    return -_INT_MAX <= n <= _INT_MAX
+
+
 class Fp8KVPool:
     """A paged 8-bit KV cache on one GPU.  `storage`, `scales` and `mass` wrap
     the caller's tensors; what is missing is allocated (mass only with
@@ -159,6 +167,8 @@ class Fp8KVPool:
         self._i32(context_lens, "context_lens", 1)
         b = context_lens.numel()
         self._i32(block_tables, "block_tables", 2, b)
+        if not _fits(max_ctx):
+            raise ValueError(f"max_ctx {max_ctx} is beyond 32 bits")
 
         def call(s: int) -> tuple[torch.Tensor, torch.Tensor]:
             shape = (b, max_ctx, self.num_kv_heads, self.head_dim)
@@ -201,6 +211,10 @@ class Fp8KVPool:
             raise ValueError(f"out must be a contiguous float32 tensor of shape {shape} on {self.device}")
         if max_ctx is None:
             max_ctx = self._longest(context_lens, int(append))
+        if window > _INT_MAX:
+            window = _INT_MAX  # longer than any sequence either way
+        if not (_fits(max_ctx) and _fits(window)):
+            raise ValueError(f"max_ctx {max_ctx}, window {window}: beyond 32 bits")
         if scale is None:
             scale = 1.0 / math.sqrt(self.head_dim)
 
@@ -245,6 +259,8 @@ class Fp8KVPool:
             raise ValueError(f"budget {budget}, recent {recent}: 0 <= recent <= budget, budget >= 1")
         if max_ctx is None:
             max_ctx = self._longest(context_lens, 0)
+        if not (_fits(max_ctx) and _fits(budget)):
+            raise ValueError(f"max_ctx {max_ctx}, budget {budget}: beyond 32 bits")
 
         def call(s: int) -> tuple[torch.Tensor, torch.Tensor]:
             kept = torch.empty((batch, self.num_kv_heads, budget), dtype=torch.int32, device=self.device)

@@ -195,3 +195,23 @@ def test_caps_too_small_for_float32_are_refused(softcap):
     assert pool.pool_status() == 0
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 63 - 1])
+def test_windows_longer_than_any_sequence(window):
+    pool = make_pool(4, 16, 2, 64, torch.Generator().manual_seed(12), scales=(-9, -6))
+    args = (torch.ones((1, 4, 64), device=DEV), i32([[0, 1]]), i32([20]))
+    assert torch.equal(pool.decode(*args, max_ctx=20, window=window), pool.decode(*args, max_ctx=20))
+
+
+def test_integers_beyond_32_bits_are_refused():
+    # not wrapped around to small ones
+    pool = make_pool(4, 16, 2, 64, torch.Generator().manual_seed(12), mass=True, scales=(-9, -6))
+    bt, cl, q = i32([[0, 1]]), i32([20]), torch.ones((1, 4, 64), device=DEV)
+    for n in (2 ** 31, 2 ** 32 + 20, -2 ** 32 + 20):
+        for bad in (lambda: pool.decode(q, bt, cl, max_ctx=n), lambda: pool.gather_kv(bt, cl, n),
+                    lambda: pool.evict(bt, cl, i32([[2]]), 16, max_ctx=n), lambda: pool.evict(bt, cl, i32([[2]]), n, max_ctx=20),
+                    lambda: pool.decode(q, bt, cl, max_ctx=20, window=-abs(n))):
+            with pytest.raises((ValueError, _lib.CloveError)):
+                bad()
+    assert pool.pool_status() == 0
+
+
