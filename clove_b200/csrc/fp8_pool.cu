@@ -11,6 +11,8 @@ namespace {
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+constexpr int kMaxEvict = 0x7fffffff - (1 << 16);
+
 int fail(int rc, const char* what) {
   set_last_error("%s", what);
   return rc;
@@ -361,6 +363,11 @@ int clove_fp8_evict(clove_fp8_pool_t pool, const int32_t* block_tables, int bt_s
   if (budget < 1 || recent < 0 || recent > budget) {
     set_last_error("fp8_evict: budget %d, recent %d (0 <= recent <= budget, budget >= 1)", budget, recent);
     return CLOVE_ERR_INVALID_ARG;
+  }
+  // the selection counts tokens and places in 32 bits, a cluster's threads at a time
+  if (budget > kMaxEvict || max_ctx > kMaxEvict) {
+    set_last_error("fp8_evict: budget %d, max_ctx %d: more than the selection counts (%d)", budget, max_ctx, kMaxEvict);
+    return CLOVE_ERR_UNSUPPORTED;
   }
   const int most = budget < max_ctx ? budget : max_ctx;
   if (new_stride <= 0 || (long long)new_stride * pool->block_size < most) {

@@ -131,7 +131,8 @@ int clove_fp8_decode(clove_fp8_pool_t pool, int dtype, const void* q, const void
  * its rows' old scales.  The new blocks must not be among the blocks the call reads.
  * kept int32 [batch, num_kv_heads, budget]: the kept tokens' old indices,
  * ascending, -1 behind the n-th; new_lens int32 [batch]: n.  Rows behind a
- * sequence's last token stay as they were.  Needs a pool with mass. */
+ * sequence's last token stay as they were.  Needs a pool with mass; budget and
+ * max_ctx are 2^31 - 2^16 - 1 at most. */
 size_t clove_fp8_evict_workspace_size(clove_fp8_pool_t pool, int batch, int max_ctx, int budget);
 int clove_fp8_evict(clove_fp8_pool_t pool, const int32_t* block_tables, int bt_stride, const int32_t* context_lens,
                     int batch, int max_ctx, const int32_t* new_tables, int new_stride, int budget, int recent,

@@ -215,3 +215,15 @@ def test_integers_beyond_32_bits_are_refused():
     assert pool.pool_status() == 0
 
 
+@pytest.mark.parametrize("budget,max_ctx", [(2 ** 31 - 1, 20), (2 ** 31 - 2 ** 16, 20), (16, 2 ** 31 - 1)])
+def test_evictions_larger_than_its_indices_count_are_refused(budget, max_ctx):
+    # refused before anything is launched: the buffers are small
+    pool = make_pool(4, 256, 2, 64, torch.Generator().manual_seed(13), mass=True)
+    bt, new = torch.zeros((1, 2 ** 23), dtype=torch.int32, device=DEV), i32([[2]])
+    kept, lens = torch.zeros(64, dtype=torch.int32, device=DEV), i32([20])
+    rc = pool._lib.clove_fp8_evict(pool.handle, bt.data_ptr(), bt.shape[1], lens.data_ptr(), 1, max_ctx, new.data_ptr(), 1,
+                                   budget, 0, kept.data_ptr(), lens.data_ptr(), None, 0, None)
+    assert rc in (_lib.ERR_INVALID_ARG, _lib.ERR_UNSUPPORTED)
+    assert pool.pool_status() == 0 and not kept.any()
+
+
