@@ -771,10 +771,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-// The power of two at or below x > 0 (within the range whose inverse is normal).
-__device__ __forceinline__ float floor_pow2(float x) {
-  return __int_as_float(min(max(__float_as_int(x) & 0x7f800000, 1 << 23), 252 << 23));
-}
 
 // kShaped: scores may be capped or biased; kKept: they are written out for the
 // weights; kTwin: groups of up to 4 queries.  A variant has none of the others'
@@ -857,7 +853,7 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 2)
       for (int i = 0; i < KJ * 16; ++i) amax = fmaxf(amax, fabsf(q[i]));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      const int e = (__float_as_int(floor_pow2(amax)) >> 23) - 127 - 13;  // divide by 2^e
+      const int e = min(max(__float_as_int(amax) >> 23, 1), 254) - 127 - 13;  // divide by 2^e
       const float up = __int_as_float((127 - max(e, -127)) << 23);
       float f = a.scale * __int_as_float((127 + max(e, -126)) << 23);
       if (e < -126) f *= 0.5f;

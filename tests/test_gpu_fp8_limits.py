@@ -120,6 +120,21 @@ def test_scales_of_each_kv_head_and_query_apart(dtype, bs, H, G, D):
     levels([900, 5000, 17], bs, H, G, D, dtype, 6, lambda j: size[j], lambda j: weight[j])
 
 
+@pytest.mark.parametrize("G,D", [(4, 128), (8, 64), (1, 256)])
+def test_queries_near_the_end_of_float32(G, D):
+    gen = torch.Generator().manual_seed(9)
+    lens = [100, 1300]
+    tables, nb = tables_for(lens, 16, gen)
+    pool = make_pool(nb, 16, 1, D, gen, scales=(-8, -5))
+    ref = RefPool(pool.storage, pool.scales)
+    q = torch.randn((2, G, D), generator=gen) * 2.0 ** 120
+    q[:, :, 3], q[:, :, 5] = torch.finfo(torch.float32).max, -torch.finfo(torch.float32).max
+    scale = 2.0 ** -126
+    want, bound = sharp_bound(ref, q, tables, lens, scale)
+    out = pool.decode(q.to(DEV), tables, i32(lens), scale=scale, max_ctx=1300)
+    assert ((out.cpu().double() - want).abs() <= bound).all()
+
+
 # ---------------------------------------------------------------------------
 # calls that run into their wait limit
 # ---------------------------------------------------------------------------
