@@ -5,16 +5,97 @@ that run into their wait limit, and what is refused.
 Outputs are held to sharp_bound, which knows no scale but those that matter:
 a block of negligible weight may not cost another one precision.
 """
-import ctypes as C
-
 import pytest
 import torch
 
 from clove_b200 import _lib
 from fp8_reference import RefPool
-from test_gpu_fp8 import DEV, F8, i32, make_pool, run_decode, tables_for
+from test_gpu_fp8 import DEV, i32, make_pool, run_decode, tables_for
 
 pytestmark = pytest.mark.gpu
+
+# ---------------------------------------------------------------------------
+# sequences that are split between CTAs
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,bs,H,G,D", [(torch.float32, 16, 2, 4, 128), (torch.float32, 64, 1, 2, 256),
+                                            (torch.float32, 256, 2, 8, 128), (torch.float16, 8, 2, 3, 64),
+                                            (torch.bfloat16, 256, 2, 1, 64), (torch.bfloat16, 32, 2, 8, 256),
+                                            (torch.float16, 128, 1, 5, 128), (torch.float32, 8, 1, 7, 64)])
+@pytest.mark.parametrize("append,accumulate", [(False, False), (True, False), (False, True), (True, True)])
+def test_long_windows(dtype, bs, H, G, D, append, accumulate):
+    # windows that start inside a block and a slice, of sequences longer and shorter than them
+    for window in (1025, 1777):
+        run_decode([3000, 1776, 0, 1777, 5, 4999, 1], bs, H, G, D, dtype, seed=window + bs + G, append=append,
+                   window=window, accumulate=accumulate, softcap=15.0 if G == 8 else 0.0, alibi=G % 2 == 1)
+
+
+@pytest.mark.parametrize("dtype,bs,H,G,D", [(torch.bfloat16, 16, 8, 2, 64), (torch.float32, 32, 6, 1, 128),
+                                            (torch.float16, 64, 5, 1, 256), (torch.bfloat16, 256, 8, 4, 64)])
+@pytest.mark.parametrize("window", [1, 33, 200, 0])
+@pytest.mark.parametrize("append,accumulate", [(False, False), (True, True)])
+def test_many_short_windows(dtype, bs, H, G, D, window, append, accumulate):
+    # more KV heads than are taken whole: short windows through the partition
+    gen = torch.Generator().manual_seed(window + bs)
+    lens = torch.randint(0, 300, (125,), generator=gen)
+    lens[::11], lens[7], lens[124] = 0, 1000, 513
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert lens.numel() * H > 4 * sms
+    run_decode(lens.tolist(), bs, H, G, D, dtype, seed=window + G, append=append, window=window, accumulate=accumulate)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bs,H,G,D", [(8, 2, 8, 128), (16, 3, 5, 64), (32, 2, 3, 256), (64, 2, 8, 256), (128, 1, 7, 128),
+                                      (256, 2, 2, 64), (256, 1, 1, 256)])
+@pytest.mark.parametrize("append", [False, True])
+def test_split_sequences(dtype, bs, H, G, D, append):
+    run_decode([0, 1, 33, 257, 2600, 1025], bs, H, G, D, dtype, seed=bs + G + D, append=append)
+
+
+# ---------------------------------------------------------------------------
+# far into a large cache
+# ---------------------------------------------------------------------------
+def test_blocks_beyond_two_gigabytes():
+    # codes of the blocks used lie beyond 2^31 bytes of their plane: what the same blocks give in a small cache
+    from clove_b200 import Fp8KVPool
+    bs, H, D, B, G = 256, 8, 128, 3, 4
+    gen = torch.Generator().manual_seed(3)
+    lens = [700, 1500, 256]
+    used = 24  # blocks 0 .. 23 of the small cache are the last ones of the large one
+    nb = 2 ** 31 // (bs * H * D) + 100
+    small, first = make_pool(used, bs, H, D, gen, mass=True), nb - used
+    assert first * bs * H * D > 2 ** 31
+    big = Fp8KVPool(nb, bs, H, D, track_mass=True)
+    big.storage.view(torch.uint8)[:, first:] = small.storage.view(torch.uint8)
+    big.scales[:, first:] = small.scales
+    big.mass[first:] = small.mass
+    ids = torch.randperm(used, generator=gen)
+    tables = torch.zeros((B, 7), dtype=torch.int32)
+    new = torch.zeros((B, 2), dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(lens):
+        k = n // bs + 1
+        tables[b, :k], at = ids[at:at + k], at + k
+    new[:] = ids[at:at + 2 * B].reshape(B, 2)
+    copies = [int(x) for x in ids[at + 2 * B:at + 2 * B + 2]]
+    kv = torch.randn((2, 300, H, D), generator=gen).bfloat16().to(DEV)
+    q = torch.randn((B, H * G, D), generator=gen).bfloat16().to(DEV)
+    slots = torch.cat([int(tables[1, 2]) * bs + torch.arange(bs), int(tables[0, 0]) * bs + torch.arange(44)])
+    got = []
+    for pool, off in ((small, 0), (big, first)):
+        t, t2 = i32(tables + off), i32(new + off)
+        pool.reshape_and_cache(kv[0], kv[1], i32(slots + off * bs))
+        outs = [pool.decode(q, t, i32(lens), max_ctx=1501, k_new=kv[0, :B], v_new=kv[1, :B], accumulate=True)]
+        outs += pool.gather_kv(t, i32([n + 1 for n in lens]), 1501)
+        outs += pool.evict(t, i32([n + 1 for n in lens]), t2, 300, 20, max_ctx=1501)
+        pool.copy_blocks(t2[:, 0].contiguous()[:2], i32([c + off for c in copies]))
+        outs += [pool.decode(q, t2, outs[-1], max_ctx=300, window=77)]
+        assert pool.pool_status() == 0
+        outs += [pool.storage.view(torch.uint8)[:, off:], pool.scales[:, off:], pool.mass[off:]]
+        got.append(outs)
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert not big.storage.view(torch.uint8)[:, :first].any()
+
 
 # ---------------------------------------------------------------------------
 # scales of any size
@@ -118,6 +199,33 @@ def test_scales_of_each_kv_head_and_query_apart(dtype, bs, H, G, D):
     size = torch.randint(-50, 50, (800,), generator=gen).tolist()
     weight = (torch.randn((800,), generator=gen) * 40).tolist()
     levels([900, 5000, 17], bs, H, G, D, dtype, 6, lambda j: size[j], lambda j: weight[j])
+
+
+# ---------------------------------------------------------------------------
+# values near the end of float32
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,bs,H,G,D", SHAPES)
+@pytest.mark.parametrize("power", [100, 116, 120])
+def test_large_values(dtype, bs, H, G, D, power):
+    # the values' sums before the division by the weights' stay finite
+    levels([700, 2600], bs, H, G, D, dtype, power, lambda j: power, lambda j: 0)
+
+
+@pytest.mark.parametrize("dtype,G,D", [(torch.bfloat16, 4, 128), (torch.float32, 8, 64), (torch.float16, 1, 256)])
+@pytest.mark.parametrize("exponent", [-149, -127, 125, 126, 127])
+def test_scales_at_the_ends_of_float32(dtype, G, D, exponent):
+    # any positive finite scale: a loaded cache's may be the smallest and the largest
+    gen = torch.Generator().manual_seed(8)
+    lens = [100, 1300]
+    tables, nb = tables_for(lens, 16, gen)
+    pool = make_pool(nb, 16, 1, D, gen, scales=(-8, -5))
+    pool.storage.view(torch.uint8)[1] &= 0x9F  # values below 2^-2
+    pool.scales[1] = 2.0 ** exponent
+    ref = RefPool(pool.storage, pool.scales)
+    q = torch.randn((2, G, D), generator=gen).to(dtype)
+    want, bound = sharp_bound(ref, q, tables, lens, 0.1)
+    out = pool.decode(q.to(DEV), tables, i32(lens), scale=0.1, max_ctx=1300)
+    assert ((out.cpu().double() - want).abs() <= bound).all()
 
 
 @pytest.mark.parametrize("G,D", [(4, 128), (8, 64), (1, 256)])
@@ -240,5 +348,3 @@ def test_evictions_larger_than_its_indices_count_are_refused(budget, max_ctx):
                                    budget, 0, kept.data_ptr(), lens.data_ptr(), None, 0, None)
     assert rc in (_lib.ERR_INVALID_ARG, _lib.ERR_UNSUPPORTED)
     assert pool.pool_status() == 0 and not kept.any()
-
-
