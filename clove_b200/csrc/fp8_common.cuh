@@ -112,7 +112,6 @@ struct Fp8DecodeCall {
   clove_fp8_scores_t scores;
   float* out;
   void* workspace;
-  size_t workspace_bytes;
 };
 
 struct Fp8EvictCall {
@@ -126,8 +125,6 @@ struct Fp8EvictCall {
   int budget, recent;
   int32_t* kept;
   int32_t* new_lens;
-  void* workspace;
-  size_t workspace_bytes;
 };
 
 // Each returns a CLOVE_* status and sets the last-error text on failure.

@@ -340,7 +340,6 @@ int clove_fp8_decode(clove_fp8_pool_t pool, int dtype, const void* q, const void
   c.scores = sc;
   c.out = out;
   c.workspace = workspace;
-  c.workspace_bytes = workspace_bytes;
   try {
     return launch_fp8_decode(*pool, c, static_cast<cudaStream_t>(stream));
   } catch (const std::exception&) {  // (the launch configurations' table)
@@ -395,8 +394,6 @@ int clove_fp8_evict(clove_fp8_pool_t pool, const int32_t* block_tables, int bt_s
   c.recent = recent;
   c.kept = kept;
   c.new_lens = new_lens;
-  c.workspace = workspace;
-  c.workspace_bytes = workspace_bytes;
   return launch_fp8_evict(*pool, c, static_cast<cudaStream_t>(stream));
 }
 
