@@ -83,10 +83,10 @@ struct Raw8 {
 // One tile of plane p by `nw` warps (32 rows each; nw = max(1, block_size /
 // 32)), this one being the w-th.  Lane r's `tok` > 0: row 32 w + r is written
 // from token tok - 1; the other rows are rounded anew if the scale grows.  D /
-// 8 lanes share a row.  `red` (3 floats per warp of the group) and barrier
+// 8 lanes share a row.  `red` (2 floats per warp of the group) and barrier
 // `bar` serve the group's maximum.  Eight 16-byte loads of a lane are
-// under way at once; where its rows are more than that they are read again,
-// from L1, to be rounded (keeping twice as many cost more in resident warps).
+// under way at once; where its rows are more than that they are read again to
+// be rounded, from L2 mostly (keeping twice as many cost more in resident warps).
 // ROWS: rows per warp (block_size, at most 32).
 template <typename T, int D, int ROWS>
 __device__ __forceinline__ void fp8_write_tile(const Fp8AppendArgs& a, int p, int blk, int h, int tok, int nw, int w, float* red, int bar,

@@ -10,18 +10,19 @@
 // Measured (heads of 128, bf16): 8 sequences of 32k to 131k tokens, 64 / 8 heads
 // 217 us (0.97 of a copy's rate; 228 to 248 in loops that reach the power
 // limit); 128 ragged sequences of 1300 tokens on average, 32 / 8 heads, with
-// append 66.5 us (0.71: start, hand-offs and combine); 256 of a window of 1024
-// with capped scores 111 us (0.67: hand-offs and instruction fetch).
+// append 66.5 us (0.72: start, hand-offs and combine); 256 of a window of 1024
+// with capped scores 113 us (0.66: hand-offs and instruction fetch).
 //
-// Mathematics.  HBM bounds this kernel, so the arithmetic is held to what
-// float32 would give instead of spending the slack elsewhere:
+// Mathematics.  HBM bounds this kernel, so its slack goes into arithmetic close
+// to float32's.  What is rounded to fewer bits than that is named:
 //   - an e4m3 code is exact in f16, so K and V enter the tensor cores exactly,
 //     and their block scales are applied to scores and weights in f32;
 //   - scores are computed transposed, K (16 tokens) times Q^T (8 queries): the
 //     m16n8k16 MMA has no row to spare.  A 16-bit query is one half once its
 //     row is scaled to the top of the f16 range (bf16 elements 2^-31 below the
 //     row's largest lose bits), an f32 query the sum of two halves and so two
-//     MMAs;
+//     MMAs: off by at most 2^-23 of itself or 2^-38 of its row's largest,
+//     where float32 has 2^-24 (a third MMA would be half as much work again);
 //   - a weight times its block's V scale is the sum of two halves, off by at
 //     most 2^-23 of itself, and the value sum is transposed too: V^T (16 dims)
 //     times P^T (8 queries).  With up to 4 queries columns 4..7 repeat queries
@@ -742,7 +743,7 @@ __device__ __forceinline__ float ex2(float x) {
 
 // tanh for |x| <= kTanhNear, where scores below a cap mostly are: x + x^3 P(x^2)
 // with P of degree 3, fitted so that the largest relative error there is
-// smallest (1.6e-8, a quarter of 2^-24; Taylor's coefficients give that up to 0.3).
+// smallest (1.6e-8, a quarter of 2^-24; Taylor's coefficients give that up to 0.26).
 constexpr float kTanhNear = 0.5f;
 __device__ __forceinline__ float2 tanh_near(float2 x) {
   const float2 y = mul2(x, x);

@@ -15,7 +15,7 @@
 // bytes per kept token and KV head (read and written, K and V) for the second.
 // Measured with 8 heads of 128, selection + moving: 128 ragged sequences (16 to
 // 8192 tokens) to 512 36 + 50 us, 8 of 32k to 131k tokens to 8192 60 + 56 us: the
-// three passes' barriers hold up the first, rows of 128 bytes gathered at
+// work and the barriers of five passes hold up the first, rows of 128 bytes gathered at
 // random (4.5 TB/s) the second.  (Launching the second early costs 12 us: its
 // CTAs take the first one's places.)
 #include <algorithm>

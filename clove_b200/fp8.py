@@ -44,7 +44,9 @@ class Fp8KVPool:
     """A paged 8-bit KV cache on one GPU.  `storage`, `scales` and `mass` wrap
     the caller's tensors; what is missing is allocated (mass only with
     track_mass).  Blocks are filled from row 0 on: a write to row 0 starts a
-    block anew, whatever an earlier sequence left in it.
+    block anew, whatever an earlier sequence left in it.  A token written to a
+    block may rewrite its other rows (to a grown scale): no other sequence or
+    call may read a block while it is appended to.
 
     Scratch comes from the caching allocator call by call, so calls on
     different streams, and graphs captured from them, share none."""
@@ -244,7 +246,8 @@ class Fp8KVPool:
               stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Bring every sequence down to min(context_lens, budget) tokens: each
         KV head keeps the last `recent` ones and the heaviest others (mass;
-        ties to the lower index), moved in order to the blocks new_tables,
+        ties to the lower index; tokens that no accumulating decode has seen
+        have mass 0, a fresh prompt's too), moved in order to the blocks new_tables,
         which must be none of the blocks the sequences hold now.  Returns
         (kept int32 [batch, num_kv_heads, budget], -1 behind the last,
         new_lens int32 [batch]).  Token indices are those of the compacted

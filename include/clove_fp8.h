@@ -10,7 +10,10 @@
  *           (K plane, V plane): a (block, KV head) tile is contiguous.
  *   scales  f32 [2, num_blocks, num_kv_heads]: an element is code * scale.
  *   mass    f32 [num_blocks, num_kv_heads, block_size], optional: the
- *           attention weight that each cached token has received.
+ *           attention weight that each cached token has received from decode
+ *           calls that accumulate.  Written tokens start at 0, prompts too:
+ *           before the first such decode an eviction finds nothing but ties
+ *           and keeps the lowest indices (and the `recent` last ones).
  *
  * Scale rule.  The scale of a (block, KV head) of a plane is 2^e with the
  * smallest e >= -126 for which 448 * 2^e covers the largest finite magnitude
@@ -34,8 +37,11 @@
  * followed, and raise CLOVE_FLAG_* in the pool's status word
  * (clove_fp8_pool_status).  No call allocates device memory or synchronises,
  * except where it says so; every call may be captured in a CUDA graph.
- * Calls on different streams may run at the same time when they write
- * different blocks and use different workspaces.
+ * Calls on different streams may run at the same time when none writes a block
+ * that another reads or writes, and they use different workspaces.  A token
+ * written to a block may rewrite the block's other rows (to a grown scale), so
+ * unlike in the 16-bit pools even a reader of earlier rows alone must not run
+ * beside it.
  */
 #ifndef CLOVE_FP8_H
 #define CLOVE_FP8_H
@@ -112,7 +118,8 @@ int clove_fp8_gather(clove_fp8_pool_t pool, const int32_t* block_tables, int bt_
  * cached tokens of each sequence, z as above.  With k_new and v_new [batch,
  * num_kv_heads, head_dim] (both or neither) the new token is appended first:
  * context_lens then holds the lengths before it, and max_ctx bounds the
- * lengths after it.  No two sequences may append to the same block.  A
+ * lengths after it.  No sequence may append to a block that another sequence of
+ * the call holds (the block manager's copy-on-write keeps forks apart).  A
  * sequence without tokens gets a zero row.  scores may be null: no cap, bias
  * or window.  The workspace needs no initialisation. */
 size_t clove_fp8_decode_workspace_size(clove_fp8_pool_t pool, int batch, int num_q_heads, int max_ctx,
@@ -128,7 +135,8 @@ int clove_fp8_decode(clove_fp8_pool_t pool, int dtype, const void* q, const void
  * the lower index).  The kept tokens move, in order, with their mass to rows
  * 0 .. n-1 of the blocks new_tables[b] (int32 [batch, new_stride], new_stride
  * * block_size >= min(budget, max_ctx)), a new block's scale being the largest of
- * its rows' old scales.  The new blocks must not be among the blocks the call reads.
+ * its rows' old scales.  The new blocks must be distinct and not among the blocks
+ * the call reads.
  * kept int32 [batch, num_kv_heads, budget]: the kept tokens' old indices,
  * ascending, -1 behind the n-th; new_lens int32 [batch]: n.  Rows behind a
  * sequence's last token stay as they were.  Needs a pool with mass; budget and
@@ -139,7 +147,9 @@ int clove_fp8_evict(clove_fp8_pool_t pool, const int32_t* block_tables, int bt_s
                     int32_t* kept, int32_t* new_lens, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Copy blocks src[i] -> dst[i] (codes, scales and mass; device int32 arrays
- * of n entries): the copies of the block manager's copy-on-write. */
+ * of n entries): the copies of the block manager's copy-on-write.  They run at
+ * the same time: a block that is written is no other copy's source or
+ * destination. */
 int clove_fp8_copy_blocks(clove_fp8_pool_t pool, const int32_t* src, const int32_t* dst, int n, void* stream);
 
 #ifdef __cplusplus
