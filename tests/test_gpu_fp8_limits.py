@@ -193,6 +193,15 @@ def test_scales_in_steps(dtype, bs, H, G, D, slope, way):
 
 
 @pytest.mark.parametrize("dtype,bs,H,G,D", SHAPES)
+@pytest.mark.parametrize("power", [-20, 0, 30, 110])
+@pytest.mark.parametrize("tilt", [-60, 0, 25])
+def test_blocks_of_zeros(dtype, bs, H, G, D, power, tilt):
+    # blocks whose values are all 0 have the smallest scale there is, 2^-126, and any weight: in front and in between
+    for n, zeros in ((700, lambda j: j < 2), (9 * bs + 1, lambda j: j % 3 == 0), (3000, lambda j: j < 5 or j % 4 == 2)):
+        levels([n], bs, H, G, D, dtype, 7, lambda j: -400 if zeros(j) else power, lambda j: tilt if zeros(j) else 0)
+
+
+@pytest.mark.parametrize("dtype,bs,H,G,D", SHAPES)
 def test_scales_of_each_kv_head_and_query_apart(dtype, bs, H, G, D):
     # random sizes and weights, independent of one another
     gen = torch.Generator().manual_seed(1)
